@@ -46,6 +46,13 @@ enum {
   MR_ERR_WORKSPACE = -6   /* workspace pointer missing or too small */
 };
 
+/* Element types of the operators that take one (`dtype` arguments). */
+enum {
+  MR_F32 = 0,
+  MR_BF16 = 1,
+  MR_F16 = 2
+};
+
 /* Library version (major*10000 + minor*100 + patch). */
 int mr_version(void);
 
@@ -537,6 +544,82 @@ int mr_peer_send(void* dst, const void* src, int64_t bytes, unsigned long long* 
 
 /* Device status word of the exchange (0 ok, MR_ERR_TIMEOUT); synchronizes. */
 int mr_peer_status(int reset);
+
+/*
+ * K10 -- rotary positions on query and key heads.  The rotary embedding of the
+ * decoder layer the reference runs inside block_output
+ * (mround/pipeline/blocks.py:578-606), for the layouts and types mr_rope_split
+ * does not take: part of a head, interleaved pairs, given positions, strided
+ * views.  For the pair of columns (j, j + r/2), or (2j, 2j + 1) when
+ * `interleaved`, j < r/2, with c and s row p of cosv / sinv (float32,
+ * (table_rows, r/2), contiguous):
+ *   transposed = 0:  y1 = x1 c - x2 s,  y2 = x1 s + x2 c
+ *   transposed = 1:  y1 = x1 c + x2 s,  y2 = x2 c - x1 s   (the gradient)
+ * in float32, rounded once to `dtype`; columns from r on are copied.
+ * p = positions[b * pos_stride + s] (int64 when positions64, else int32), or s
+ * when positions is NULL; a position outside [0, table_rows) writes NaN to the
+ * rotated columns.  q and k (k may be NULL) describe heads of d columns
+ * (columns contiguous, the other strides in elements); y may be x.
+ * 1 <= d <= 1024, r even, 2 <= r <= d.  Any alignment of the element type;
+ * 16-byte aligned data and strides take 16-byte accesses.
+ */
+typedef struct mr_rotary_heads {
+  const void* x;
+  void* y;
+  int64_t x_batch, x_pos, x_head;
+  int64_t y_batch, y_pos, y_head;
+  int heads;
+} mr_rotary_heads;
+
+int mr_rotary(const mr_rotary_heads* q, const mr_rotary_heads* k, const float* cosv,
+              const float* sinv, int64_t table_rows, const void* positions, int positions64,
+              int64_t pos_stride, int64_t b, int s, int d, int r, int interleaved, int transposed,
+              int dtype, void* stream);
+
+/*
+ * The block's operand forms of K10: mr_rope_split / mr_rope_bwd_split for a
+ * rotated part of r columns (tables (s, r/2)) and either layout.  Same tensors
+ * as there; d and r even.
+ */
+int mr_rotary_split(const float* qkv, const float* cosv, const float* sinv, int b, int s, int hq,
+                    int hkv, int d, int r, int interleaved, uint16_t* q_hi, uint16_t* q_lo,
+                    uint16_t* k_hi, uint16_t* k_lo, uint16_t* v_hi, uint16_t* v_lo, void* stream);
+int mr_rotary_bwd_split(const float* dq, const float* dk, const float* dv, const float* cosv,
+                        const float* sinv, int b, int s, int hq, int hkv, int d, int r,
+                        int interleaved, uint16_t* hi, uint16_t* lo, float* t32, void* stream);
+
+/*
+ * K11 -- the k largest values of each row of `logits` ((rows, n), row stride
+ * ld elements, any alignment of the type) with their columns, in descending
+ * order: NaN first, equal values (+0 and -0 too) by lowest column.  No
+ * counterpart in the reference, whose scoring knows hard labels only
+ * (mround/pipeline/scoring.py:183-192): it captures the teacher's top logits
+ * for mr_distill_topk.  values float32, indices int64, both (rows, k).
+ * 1 <= k <= min(n, 256).
+ */
+int mr_topk_logits(const void* logits, int64_t rows, int n, int64_t ld, int k, int dtype,
+                   float* values, int64_t* indices, void* stream);
+
+/*
+ * K12 -- distillation from a teacher's top logits, loss and/or gradient.  The
+ * objective of a scoring backward against a teacher instead of the hard labels
+ * of _causal_loss (mround/pipeline/scoring.py:183-192).  Per row, with the
+ * teacher's t_logits (float32) at columns t_index (int64), both (rows, k):
+ *   p = softmax(t_logits / temperature) over the kept entries (t_index >= 0)
+ *   q = softmax(logits / temperature) over all n columns
+ *   loss = weight * temperature^2 * sum p (log p - log q[t_index])
+ *   grad = weight * temperature * (q - p scattered to its columns)
+ * A column that occurs twice counts twice.  A row of zero weight, or without a
+ * kept entry, gives zero loss and gradient whatever it holds; a column >= n
+ * gives NaN in that row.  weight NULL: 1.  logits (rows, n), row stride ld, of
+ * `dtype`.  Outputs, any may be NULL: loss float32 (rows); the gradient either
+ * as `dtype` in grad (may be logits itself, with ldg = ld) or as a bf16 pair
+ * grad_hi / grad_lo, row stride ldg.  1 <= k <= 256.
+ */
+int mr_distill_topk(const void* logits, int64_t rows, int n, int64_t ld, int dtype,
+                    const float* t_logits, const int64_t* t_index, int k, double temperature,
+                    const float* weight, float* loss, void* grad, uint16_t* grad_hi,
+                    uint16_t* grad_lo, int64_t ldg, void* stream);
 
 #ifdef __cplusplus
 }

@@ -92,6 +92,12 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mr_ce_grad_split": (_I, [_P, _P, _I64, _I, _F, _P, _P, _P]),
     "mr_softmax_causal_split": (_I, [_P, _I64, _I, _F, _I, _P, _P, _P]),
     "mr_softmax_bwd_split": (_I, [_P, _P, _P, _I64, _I, _F, _I, _P, _P, _P]),
+    "mr_topk_logits": (_I, [_P, _I64, _I, _I64, _I, _I, _P, _P, _P]),
+    "mr_distill_topk": (_I, [_P, _I64, _I, _I64, _I, _P, _P, _I, _D, _P, _P, _P, _P, _P, _I64,
+                             _P]),
+    "mr_rotary": (_I, [_P, _P, _P, _P, _I64, _P, _I, _I64, _I64, _I, _I, _I, _I, _I, _I, _P]),
+    "mr_rotary_split": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
+    "mr_rotary_bwd_split": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P]),
 }
 
 
@@ -103,6 +109,15 @@ class K2Segment(ctypes.Structure):
         ("init_scale", _P), ("rows", _I64), ("cols", _I64), ("bits", _I), ("lr", _F),
         ("coef_lo", _F), ("coef_hi", _F), ("wq_hi", _P), ("wq_lo", _P), ("wq_t32", _P),
         ("codes", _P), ("qscale", _P), ("qzp", _P),
+    ]
+
+
+class RotaryHeads(ctypes.Structure):
+    """``mr_rotary_heads``: the query or key heads of an ``mr_rotary`` launch."""
+
+    _fields_ = [
+        ("x", _P), ("y", _P), ("x_batch", _I64), ("x_pos", _I64), ("x_head", _I64),
+        ("y_batch", _I64), ("y_pos", _I64), ("y_head", _I64), ("heads", _I),
     ]
 
 

@@ -17,6 +17,8 @@ __all__ = [
     "LossWorkspace",
     "colsumsq_split",
     "deltaloss",
+    "distill_topk",
+    "distill_topk_grad",
     "fq_forward",
     "gemm",
     "gemm_batched",
@@ -26,10 +28,13 @@ __all__ = [
     "loss_outlier",
     "loss_select_digit",
     "pack_mlx",
+    "rotary",
+    "rotary_bwd",
     "round_tf32",
     "scale_search",
     "split_bf16",
     "ste_signsgd",
+    "topk_logits",
 ]
 
 DEVICE_GROUPS = (8, 16, 32, 64, 128, 256)
@@ -603,11 +608,31 @@ def rmsnorm_bwd_split(dy, x, w, rstd, resid, *, split: bool = True, t32: bool = 
     return hi, lo, tt
 
 
-def rope_split(qkv, cos, sin, b: int, s: int, hq: int, hkv: int, d: int):
+def _whole_half(layout: str, rotary_dim, d: int) -> bool:
+    """Whether the rotation is the half layout over the whole head."""
+    _interleaved(layout)
+    return layout == "half" and rotary_dim in (None, d)
+
+
+def rope_split(qkv, cos, sin, b: int, s: int, hq: int, hkv: int, d: int, *, layout: str = "half",
+               rotary_dim: int | None = None):
+    """qkv rows -> rope(q), rope(k), v as (B, H, S, D) hi/lo pairs.  ``rotary_dim``: the
+    head's rotated columns (tables (s, rotary_dim / 2)), the whole head by default."""
     dev = qkv.device
     q = _pair((b, hq, s, d), dev)
     k = _pair((b, hkv, s, d), dev)
     v = _pair((b, hkv, s, d), dev)
+    if not _whole_half(layout, rotary_dim, d):
+        r = d if rotary_dim is None else rotary_dim
+        st = lib().mr_rotary_split(_ptr(qkv, torch.float32, "qkv", b * s * (hq + 2 * hkv) * d),
+                                   _ptr(cos, torch.float32, "cos", s * r // 2),
+                                   _ptr(sin, torch.float32, "sin", s * r // 2), b, s, hq, hkv, d,
+                                   r, _interleaved(layout), q[0].data_ptr(), q[1].data_ptr(),
+                                   k[0].data_ptr(), k[1].data_ptr(), v[0].data_ptr(),
+                                   v[1].data_ptr(), _stream())
+        check(st, "mr_rotary_split")
+        _count()
+        return q, k, v
     st = lib().mr_rope_split(_ptr(qkv, torch.float32, "qkv", b * s * (hq + 2 * hkv) * d),
                              _ptr(cos, torch.float32, "cos", s * d // 2),
                              _ptr(sin, torch.float32, "sin", s * d // 2), b, s, hq, hkv, d,
@@ -619,11 +644,24 @@ def rope_split(qkv, cos, sin, b: int, s: int, hq: int, hkv: int, d: int):
 
 
 def rope_bwd_split(dq, dk, dv, cos, sin, b: int, s: int, hq: int, hkv: int, d: int, *,
-                   split: bool = True, t32: bool = False):
+                   split: bool = True, t32: bool = False, layout: str = "half",
+                   rotary_dim: int | None = None):
     """The qkv-row gradient as (hi, lo, tf32 copy), None for what was not asked."""
     shape = (b * s, (hq + 2 * hkv) * d)
     hi, lo = _pair(shape, dq.device) if split else (None, None)
     tt = _t32(shape, dq.device, t32)
+    if not _whole_half(layout, rotary_dim, d):
+        r = d if rotary_dim is None else rotary_dim
+        nq, nkv = b * s * hq * d, b * s * hkv * d
+        st = lib().mr_rotary_bwd_split(
+            _ptr(dq, torch.float32, "dq", nq), _ptr(dk, torch.float32, "dk", nkv),
+            _ptr(dv, torch.float32, "dv", nkv), _ptr(cos, torch.float32, "cos", s * r // 2),
+            _ptr(sin, torch.float32, "sin", s * r // 2), b, s, hq, hkv, d, r, _interleaved(layout),
+            None if hi is None else hi.data_ptr(), None if lo is None else lo.data_ptr(),
+            _ptr(tt, torch.float32, "t32", shape[0] * shape[1]), _stream())
+        check(st, "mr_rotary_bwd_split")
+        _count()
+        return hi, lo, tt
     st = lib().mr_rope_bwd_split(_ptr(dq, torch.float32, "dq"), _ptr(dk, torch.float32, "dk"),
                                  _ptr(dv, torch.float32, "dv"), _ptr(cos, torch.float32, "cos"),
                                  _ptr(sin, torch.float32, "sin"), b, s, hq, hkv, d,
@@ -721,3 +759,234 @@ def softmax_bwd_split(dp, p, rows: int, s: int, scale: float, band: bool = False
     check(st, "mr_softmax_bwd_split")
     _count()
     return hi, lo
+
+
+# ------------------------------------------------- rotary, logits and linear operators
+# Unlike the functions above, these take tensors of any CUDA device and launch
+# on that device's current stream.
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _interleaved(layout: str) -> int:
+    if layout not in ("half", "interleaved"):
+        raise SchemeError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    return int(layout == "interleaved")
+
+
+def _device_of(**tensors) -> torch.device:
+    """The CUDA device all given tensors share."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise PlatformError(f"{name} must be a CUDA tensor (there is no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise SchemeError(f"{name} is on {t.device}, expected {dev}")
+    return dev
+
+
+def _launch(name: str, dev: torch.device, *args) -> None:
+    """One C entry point on ``dev``'s current stream (appended to ``args``)."""
+    fn = getattr(lib(), name)
+    if dev.index == torch.cuda.current_device():
+        status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    check(status, name)
+    _count()
+
+
+def _dtype_code(t: torch.Tensor, name: str) -> int:
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise SchemeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _rotary(q, k, cos, sin, positions, layout, out, transposed):
+    from mround_b200._native import RotaryHeads
+
+    inter = _interleaved(layout)
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise SchemeError("q and k are (batch, positions, heads, head dim)")
+    b, s, hq, d = q.shape
+    if out is None:
+        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+               None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
+    yq, yk = out
+    dev = _device_of(q=q, k=k, cos=cos, sin=sin, positions=positions, out_q=yq, out_k=yk)
+    code = _dtype_code(q, "q")
+    if (k is None) != (yk is None):
+        raise SchemeError("out is a (q, k) pair with k None exactly where k is")
+    for name, x, y in (("q", q, yq), ("k", k, yk)):
+        if x is None:
+            continue
+        if x.dtype != q.dtype or y.dtype != q.dtype:
+            raise SchemeError(f"{name} and its output must be {q.dtype}")
+        if x.shape[:2] != (b, s) or x.shape[3] != d or y.shape != x.shape:
+            raise SchemeError(f"{name} has shape {tuple(x.shape)} and output {tuple(y.shape)}, "
+                              f"expected ({b}, {s}, heads, {d})")
+        if (x.stride(3) != 1 or y.stride(3) != 1) and d > 1:
+            raise SchemeError(f"{name}'s last dimension must be contiguous")
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        raise SchemeError(f"cos and sin are (positions, rotated columns / 2) tables, got "
+                          f"{tuple(cos.shape)} and {tuple(sin.shape)}")
+    rows, half = cos.shape
+    if not 1 <= half <= d // 2 or d > 1024:
+        raise SchemeError(f"tables of {half} pairs do not fit head dim {d} (at most 1024)")
+    pos_ptr, pos64, pos_stride = None, 0, 0
+    if positions is not None:
+        if positions.dtype not in (torch.int64, torch.int32):
+            raise SchemeError(f"positions must be int64 or int32, got {positions.dtype}")
+        if positions.shape not in ((s,), (b, s)) or not positions.is_contiguous():
+            raise SchemeError(f"positions must be a contiguous ({s},) or ({b}, {s}) tensor")
+        pos_ptr, pos64 = positions.data_ptr(), int(positions.dtype == torch.int64)
+        pos_stride = s if positions.dim() == 2 else 0
+    elif s > rows:
+        raise SchemeError(f"{s} positions but tables of {rows} rows")
+    if hq == 0 or (k is not None and k.shape[2] == 0):
+        raise SchemeError("q and k need at least one head")
+    if b * s == 0:
+        return out
+    heads = [None, None]
+    for i, (x, y) in enumerate(((q, yq), (k, yk))):
+        if x is not None:
+            sx, sy = x.stride(), y.stride()
+            heads[i] = RotaryHeads(x.data_ptr(), y.data_ptr(), sx[0], sx[1], sx[2], sy[0], sy[1],
+                                   sy[2], x.shape[2])
+    _launch("mr_rotary", dev, _ref(heads[0]), _ref(heads[1]), _ptr(cos, torch.float32, "cos"),
+            _ptr(sin, torch.float32, "sin"), rows, pos_ptr, pos64, pos_stride, b, s, d, 2 * half,
+            inter, transposed, code)
+    return out
+
+
+def _ref(struct):
+    import ctypes
+
+    return None if struct is None else ctypes.addressof(struct)
+
+
+def rotary(q, k, cos, sin, *, positions=None, layout: str = "half", out=None):
+    """K10: rotary positions on ``q`` (B, S, Hq, D) and ``k`` (B, S, Hkv, D) or None.
+
+    float32, bfloat16 or float16 (computed in float32, rounded once); any
+    strides with contiguous columns, so views of a fused projection or of
+    (B, H, S, D) storage need no copy.  ``cos`` / ``sin``: float32 (rows,
+    r / 2) tables as :func:`mround_b200.pipeline.block.rope_tables` makes them;
+    the head's first r columns turn, the rest are copied.  ``layout``: pairs
+    (j, j + r/2) for "half", (2j, 2j + 1) for "interleaved".  ``positions``:
+    int32 or int64 (S,) or (B, S) table rows, 0..S-1 by default; a position
+    outside the tables gives NaN.  ``out``: a (q, k) pair of tensors to write,
+    which may be ``q`` and ``k`` themselves.  Returns (q, k) turned."""
+    return _rotary(q, k, cos, sin, positions, layout, out, 0)
+
+
+def rotary_bwd(dq, dk, cos, sin, *, positions=None, layout: str = "half", out=None):
+    """Gradients of :func:`rotary`'s inputs from those of its outputs (the
+    transposed rotation; same arguments)."""
+    return _rotary(dq, dk, cos, sin, positions, layout, out, 1)
+
+
+MAX_TOPK = 256
+
+
+def _logit_rows(logits):
+    """(rows, columns, row stride) of a 2-D tensor with contiguous columns."""
+    if logits.dim() != 2:
+        raise SchemeError(f"logits are (rows, vocabulary), got shape {tuple(logits.shape)}")
+    rows, n = logits.shape
+    if n == 0 or (n > 1 and logits.stride(1) != 1) or n > 0x7FFFFFFF:
+        raise SchemeError("the logits' columns must be contiguous, at least one")
+    ld = logits.stride(0) if rows > 1 else n
+    if ld < n:
+        raise SchemeError("the logits' rows overlap")
+    return rows, n, ld
+
+
+def topk_logits(logits, k: int):
+    """K11: the ``k`` largest logits of each row and their columns, in descending
+    order with equal values by lowest column (NaN counts as the largest).
+
+    ``logits``: (rows, vocabulary) float32, bfloat16 or float16, contiguous
+    columns.  1 <= k <= min(vocabulary, 256).  Returns float32 values and int64
+    columns, (rows, k) each -- what :func:`distill_topk` takes."""
+    dev = _device_of(logits=logits)
+    rows, n, ld = _logit_rows(logits)
+    code = _dtype_code(logits, "logits")
+    if not 1 <= k <= min(n, MAX_TOPK):
+        raise SchemeError(f"k must be 1 to {min(n, MAX_TOPK)}, got {k}")
+    values = torch.empty((rows, k), dtype=torch.float32, device=dev)
+    index = torch.empty((rows, k), dtype=torch.int64, device=dev)
+    if rows:
+        _launch("mr_topk_logits", dev, logits.data_ptr(), rows, n, ld, k, code, values.data_ptr(),
+                index.data_ptr())
+    return values, index
+
+
+def _distill(logits, t_logits, t_index, temperature, weight, loss, grad, pair, ldg):
+    dev = _device_of(logits=logits, t_logits=t_logits, t_index=t_index, weight=weight, out=grad,
+                     out_hi=pair[0], out_lo=pair[1])
+    rows, n, ld = _logit_rows(logits)
+    code = _dtype_code(logits, "logits")
+    if t_logits.dim() != 2 or t_logits.shape != t_index.shape or t_logits.shape[0] != rows:
+        raise SchemeError(f"t_logits and t_index are ({rows}, k), got {tuple(t_logits.shape)} and "
+                          f"{tuple(t_index.shape)}")
+    k = t_logits.shape[1]
+    if not 1 <= k <= MAX_TOPK:
+        raise SchemeError(f"1 to {MAX_TOPK} teacher logits per row, got {k}")
+    if not 0.0 < float(temperature) < 1e30:
+        raise SchemeError(f"temperature must be positive, got {temperature}")
+    args = (_ptr(t_logits, torch.float32, "t_logits"), _ptr(t_index, torch.int64, "t_index"), k,
+            float(temperature), _ptr(weight, torch.float32, "weight", rows))
+    if rows:
+        _launch("mr_distill_topk", dev, logits.data_ptr(), rows, n, ld, code, *args,
+                None if loss is None else loss.data_ptr(),
+                None if grad is None else grad.data_ptr(),
+                None if pair[0] is None else pair[0].data_ptr(),
+                None if pair[1] is None else pair[1].data_ptr(), ldg)
+
+
+def distill_topk(logits, t_logits, t_index, *, temperature: float = 1.0, weight=None):
+    """K12, the loss alone: per row, ``weight * T^2 * KL(p || q)`` with
+    ``p = softmax(t_logits / T)`` over the teacher's kept logits and
+    ``q = softmax(logits / T)`` over the whole vocabulary.
+
+    ``logits``: (rows, vocabulary) float32, bfloat16 or float16, contiguous
+    columns.  ``t_logits`` float32 and ``t_index`` int64, (rows, k), k <= 256: a
+    negative column is an absent entry, a repeated one counts as often as it
+    occurs, one beyond the vocabulary makes its row NaN.  ``weight``: float32
+    (rows,); a row of weight 0, or without an entry, gives 0 whatever it holds.
+    Returns float32 (rows,)."""
+    loss = torch.empty(logits.shape[:1], dtype=torch.float32, device=logits.device)
+    _distill(logits, t_logits, t_index, temperature, weight, loss, None, (None, None), 0)
+    return loss
+
+
+def distill_topk_grad(logits, t_logits, t_index, *, temperature: float = 1.0, weight=None,
+                      out=None, split: bool = False):
+    """K12, the loss and its gradient in one launch: arguments of
+    :func:`distill_topk`; the gradient is that of the losses' sum with respect
+    to ``logits`` (an upstream gradient per row goes into ``weight``).
+
+    The gradient has the logits' type, in ``out`` when given (contiguous
+    columns; ``logits`` itself may be given), or with ``split`` is the bf16
+    (hi, lo) pair that :func:`gemm` takes.  Returns (loss, gradient)."""
+    loss = torch.empty(logits.shape[:1], dtype=torch.float32, device=logits.device)
+    if split:
+        if out is not None:
+            raise SchemeError("a split gradient is allocated by the call")
+        pair = _pair(logits.shape, logits.device)
+        _distill(logits, t_logits, t_index, temperature, weight, loss, None, pair,
+                 logits.shape[-1])
+        return loss, pair
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype:
+        raise SchemeError(f"out must be {tuple(logits.shape)} {logits.dtype}")
+    _, _, ldg = _logit_rows(out)
+    _distill(logits, t_logits, t_index, temperature, weight, loss, out, (None, None), ldg)
+    return loss, out
