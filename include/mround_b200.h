@@ -458,8 +458,8 @@ int mr_gemm_tile_n(int64_t m, int64_t n, int64_t k, int64_t batch, int precision
 int mr_gemm_tile_m(int64_t m, int64_t n, int64_t k, int64_t batch, int precision, int a_kmajor,
                    int b_kmajor, int causal);
 
-/* Device status word of K3: 0, or MR_ERR_TIMEOUT.  Synchronizes the device;
- * reset != 0 clears it. */
+/* Device status word of K3 and K13: 0, or MR_ERR_TIMEOUT.  Synchronizes the
+ * device; reset != 0 clears it. */
 int mr_gemm_status(int reset);
 
 /*
@@ -620,6 +620,63 @@ int mr_distill_topk(const void* logits, int64_t rows, int n, int64_t ld, int dty
                     const float* t_logits, const int64_t* t_index, int k, double temperature,
                     const float* weight, float* loss, void* grad, uint16_t* grad_hi,
                     uint16_t* grad_lo, int64_t ldg, void* stream);
+
+/*
+ * K13 -- matrix product with bias, activation and residual in its epilogue.  A
+ * linear of the decoder block (mround/pipeline/runner.py:364-367) with what
+ * follows it in the layer (mround/pipeline/blocks.py:578-606):
+ *   z[t, f] = sum_k x[t, k] w[f, k] + bias[f]
+ *   out[t, f] = act(z)[t, f] + residual[t, f]
+ * act: none, SiLU z / (1 + e^-z), GELU z Phi(z), its tanh form, or SwiGLU,
+ * where w has 2 * feats rows [gate | up], out = silu(z_gate) * z_up.
+ * Operands are bf16: hi alone, or hi and lo parts (w a pair only with x a
+ * pair); one, two or three products as in mr_gemm, float32 accumulation.
+ * kmajor = 1: element (row, k) at hi[row * ld + k]; 0: at hi[k * ld + row]
+ * (not for a SwiGLU w).  ld a multiple of 8, data 16-byte aligned.
+ * bias: float32 (rows of w) or NULL.  residual: (toks, feats) MR_F32 or
+ * MR_BF16, row stride ldr, may be out's storage, or NULL.  out: MR_F32 or
+ * MR_BF16, row stride ldo; out_lo (with MR_BF16): the bf16 part out leaves;
+ * out_t32: the value rounded to tf32; pre: z in float32 (toks, rows of w), row
+ * stride ldp, for mr_act_grad -- each may be NULL.
+ * splits: 0 lets the call divide k among 1, 2, 4 or 8 CTAs where that fills
+ * the device (fewer rounding steps in one order per divisor, all of them
+ * reproducible); 1, 2, 4, 8 fix the divisor.  With splits = 1 a token's
+ * result does not depend on the other tokens of the call.  Device-side waits
+ * are bounded; a wait that gives up is reported by mr_gemm_status.
+ */
+enum {
+  MR_ACT_NONE = 0,
+  MR_ACT_SILU = 1,
+  MR_ACT_GELU = 2,
+  MR_ACT_GELU_TANH = 3,
+  MR_ACT_SWIGLU = 4
+};
+
+typedef struct mr_linear_operand {
+  const uint16_t* hi;
+  const uint16_t* lo;
+  int64_t ld;
+  int kmajor;
+} mr_linear_operand;
+
+int mr_linear(const mr_linear_operand* x, const mr_linear_operand* w, int64_t toks, int64_t feats,
+              int64_t k, int act, const float* bias, const void* residual, int residual_dtype,
+              int64_t ldr, void* out, int out_dtype, uint16_t* out_lo, float* out_t32, int64_t ldo,
+              float* pre, int64_t ldp, int splits, void* stream);
+
+/*
+ * The element-wise part of K13's backward: dz = dy * act'(z) as a bf16 pair
+ * (toks, feats; twice as many columns [gate | up] under SwiGLU), row stride
+ * ldo, the operand of the gradient products mr_linear forms from it (dx = dz w,
+ * dw = dz^T x), and bias_grad = sum over tokens of dz (float32, or NULL).  dy
+ * MR_F32 or MR_BF16, z the `pre` of mr_linear (NULL where act is none).  The bias gradient needs a
+ * workspace of mr_act_grad_workspace_bytes, which must not be shared by calls
+ * that may overlap.  At most 65535 * 64 tokens.
+ */
+size_t mr_act_grad_workspace_bytes(int64_t toks, int64_t feats, int act);
+int mr_act_grad(const void* dy, int dy_dtype, int64_t ldy, const float* z, int64_t ldz,
+                int64_t toks, int64_t feats, int act, uint16_t* hi, uint16_t* lo, int64_t ldo,
+                float* bias_grad, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

@@ -92,6 +92,10 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mr_ce_grad_split": (_I, [_P, _P, _I64, _I, _F, _P, _P, _P]),
     "mr_softmax_causal_split": (_I, [_P, _I64, _I, _F, _I, _P, _P, _P]),
     "mr_softmax_bwd_split": (_I, [_P, _P, _P, _I64, _I, _F, _I, _P, _P, _P]),
+    "mr_linear": (_I, [_P, _P, _I64, _I64, _I64, _I, _P, _P, _I, _I64, _P, _I, _P, _P, _I64, _P,
+                       _I64, _I, _P]),
+    "mr_act_grad_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I]),
+    "mr_act_grad": (_I, [_P, _I, _I64, _P, _I64, _I64, _I64, _I, _P, _P, _I64, _P, _P, _P]),
     "mr_topk_logits": (_I, [_P, _I64, _I, _I64, _I, _I, _P, _P, _P]),
     "mr_distill_topk": (_I, [_P, _I64, _I, _I64, _I, _P, _P, _I, _D, _P, _P, _P, _P, _P, _I64,
                              _P]),
@@ -110,6 +114,12 @@ class K2Segment(ctypes.Structure):
         ("coef_lo", _F), ("coef_hi", _F), ("wq_hi", _P), ("wq_lo", _P), ("wq_t32", _P),
         ("codes", _P), ("qscale", _P), ("qzp", _P),
     ]
+
+
+class LinearOperand(ctypes.Structure):
+    """``mr_linear_operand``: one operand of an ``mr_linear`` product."""
+
+    _fields_ = [("hi", _P), ("lo", _P), ("ld", _I64), ("kmajor", _I)]
 
 
 class RotaryHeads(ctypes.Structure):

@@ -1,0 +1,518 @@
+// K13 -- matrix product with bias, activation and residual in its epilogue,
+// on the tcgen05 tensor cores (sm_100a).
+//
+//   z[t, f] = sum_k x[t, k] w[f, k] + bias[f]
+//   y = act(z)  (none, SiLU, GELU by erf or tanh; SwiGLU: the features are
+//   [gate | up] and y = silu(z_gate) z_up)      out = y + residual
+//
+// Operands are bf16, each either one tensor or a hi/lo pair (x = hi + lo), as
+// in K3: one, two (x a pair) or three (both pairs) products into one float32
+// accumulator, per 16 k in the order x_hi w_hi, x_hi w_lo, x_lo w_hi.  Either
+// operand may be K-major or MN-major, which makes the two gradient products of
+// a linear the same kernel.
+//
+// The features are the MMA's M and the tokens its N.  An accumulator lane is
+// then one feature: the bias is one register per thread, a warp's store is 32
+// neighbouring features of one token, and N shrinks with the tokens (16 for a
+// single one) while the weights keep all 128 lanes busy -- few tokens cost one
+// reading of the weights.  SwiGLU takes 64 gate rows and the 64 up rows of the
+// same features into one 128-row tile.
+//
+// split kernel: one tile of 128 features x BT tokens per CTA, K divided among
+// the CTAs of a cluster.  Each leaves its float32 partial tile in its own
+// shared memory; the cluster's CTAs then each finish a share of the tokens,
+// reading the partials over distributed shared memory in rank order, so the
+// result does not depend on timing and needs no workspace.
+//
+// Roles (256 threads): warp 0 one lane TMA producer; warp 1 TMEM and one lane
+// MMA issuer; warps 2-5 read the accumulator; all warps finish the outputs.
+// Every mbarrier wait is bounded: one that gives up sets the status word that
+// mr_gemm_status reads, and every role goes on to the barriers at the end.
+
+#include <string.h>
+
+#include "linear.h"
+#include "rowtypes.cuh"
+#include "sm100.cuh"
+
+namespace mr {
+namespace {
+
+constexpr int kBK = 64;                // K per stage: 128-byte rows
+constexpr int kTileF = 128;            // accumulator lanes per CTA
+constexpr int kABytes = kTileF * kBK * 2;
+constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s per wait
+
+__device__ int g_linear_status = 0;
+
+// Bounded wait; returns false (and raises the status word) on timeout.
+__device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u) {
+      if (globaltimer() - t0 > kWaitLimitNs) {
+        atomicExch(&g_linear_status, MR_ERR_TIMEOUT);
+        return false;
+      }
+      if (*reinterpret_cast<volatile int*>(&g_linear_status) != 0) return false;
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+struct LinMaps {
+  CUtensorMap a_hi, a_lo, b_hi, b_lo;  // a: features, b: tokens
+  int a_kmajor, b_kmajor;
+};
+
+// What follows the product.  feats counts outputs (half of the features under
+// SwiGLU, whose up rows start at row `feats`).
+struct LinEpilogue {
+  const float* bias;
+  const void* residual;
+  void* out;
+  uint16_t* lo;
+  float* t32;
+  float* pre;
+  int64_t ldr, ldo, ldp;
+  int residual_dtype, out_dtype, act, feats, toks;
+};
+
+// silu as the block's element-wise kernels compute it
+__device__ __forceinline__ float silu1(float g) { return g / (1.f + expf(-g)); }
+
+__device__ __forceinline__ float act1(float z, int act) {
+  switch (act) {
+    case MR_ACT_SILU: return silu1(z);
+    case MR_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case MR_ACT_GELU_TANH:
+      return 0.5f * z * (1.f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
+    default: return z;
+  }
+}
+
+// One output: feature f, token t, z without bias (zu: the up row's, SwiGLU).
+template <bool kGated>
+__device__ __forceinline__ void finish(const LinEpilogue& e, int f, int t, float z, float zu) {
+  if (e.bias) {
+    z += e.bias[f];
+    if (kGated) zu += e.bias[e.feats + f];
+  }
+  if (e.pre) {
+    e.pre[int64_t(t) * e.ldp + f] = z;
+    if (kGated) e.pre[int64_t(t) * e.ldp + e.feats + f] = zu;
+  }
+  float y = kGated ? silu1(z) * zu : act1(z, e.act);
+  if (e.residual) {
+    const int64_t at = int64_t(t) * e.ldr + f;
+    y += e.residual_dtype == MR_F32 ? static_cast<const float*>(e.residual)[at]
+                                    : bf16_to_f32(static_cast<const uint16_t*>(e.residual)[at]);
+  }
+  const int64_t at = int64_t(t) * e.ldo + f;
+  if (e.out_dtype == MR_F32) {
+    static_cast<float*>(e.out)[at] = y;
+  } else {
+    const uint16_t h = f32_to_bf16(y);
+    static_cast<uint16_t*>(e.out)[at] = h;
+    if (e.lo) e.lo[at] = f32_to_bf16(__fsub_rn(y, bf16_to_f32(h)));
+  }
+  if (e.t32) e.t32[at] = tf32_rna(y);
+}
+
+// bf16 x bf16 -> float32
+__host__ __device__ constexpr uint32_t lin_idesc(int m, int n, bool a_mn, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) |
+         (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+
+// 128-byte-swizzled tiles.  K-major: rows of 64 k, 8-row groups 1024 B apart,
+// 16 k are 32 B.  MN-major: boxes of 64 columns x 64 k (8 KB), 8-k groups
+// 1024 B apart, 16 k are 2048 B.
+__device__ __forceinline__ uint64_t lin_desc(uint32_t base, bool kmajor, int ks) {
+  return kmajor ? smem_desc(base + ks * 32, 16, 1024, 2)
+                : smem_desc(base + ks * 2048, 64 * kBK * 2, 1024, 2);
+}
+
+template <int BT, int PREC>
+struct SplitCfg {
+  static constexpr int kAParts = PREC == 3 ? 2 : 1;
+  static constexpr int kBParts = PREC >= 2 ? 2 : 1;
+  static constexpr int kBBytes = BT * kBK * 2;
+  static constexpr int kStage = kABytes * kAParts + kBBytes * kBParts;
+  // two CTAs per SM where four stages fit half of its shared memory
+  static constexpr int kBudget = kStage * 4 <= 104 * 1024 ? 104 * 1024 : 208 * 1024;
+  static constexpr int kStages = kBudget / kStage > 8 ? 8 : kBudget / kStage;
+  static constexpr int kPartial = BT * kTileF * 4;  // reuses the stages
+  static constexpr int kSmem = kStages * kStage + 1024 /* align */ + 256 /* barriers */;
+  static constexpr int kTmemCols = BT < 32 ? 32 : BT;
+  static_assert(kStages * kStage >= kPartial, "the partial tile must fit the stages");
+};
+
+constexpr int kSplitThreads = 256;
+
+// One stage of a tile: features from f0 (SwiGLU: 64 gate rows and their up
+// rows), tokens from t0, k from k0.
+template <int ROWS>
+__device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* map, uint64_t* bar,
+                                          bool kmajor, int row0, int k0) {
+  if (kmajor) {
+    tma_load_3d(dst, map, bar, k0, row0, 0);
+  } else {
+#pragma unroll
+    for (int c = 0; c < ROWS / 64; ++c)
+      tma_load_3d(dst + c * 64 * kBK * 2, map, bar, row0 + c * 64, k0, 0);
+  }
+}
+
+template <bool kGated>
+__device__ __forceinline__ void load_features(uint8_t* dst, const CUtensorMap* map, uint64_t* bar,
+                                              bool kmajor, int f0, int up0, int k0) {
+  if constexpr (kGated) {
+    tma_load_3d(dst, map, bar, k0, f0, 0);
+    tma_load_3d(dst + kABytes / 2, map, bar, k0, up0 + f0, 0);
+  } else {
+    load_rows<kTileF>(dst, map, bar, kmajor, f0, k0);
+  }
+}
+
+template <int BT, int PREC, bool kGated>
+__global__ void __launch_bounds__(kSplitThreads)
+    linear_split_kernel(const __grid_constant__ LinMaps maps,
+                        const __grid_constant__ LinEpilogue e, int k, int splits, int f_tiles) {
+  using C = SplitCfg<BT, PREC>;
+  constexpr int kOut = kGated ? kTileF / 2 : kTileF;  // outputs per tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStage);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* done = empty + C::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = splits > 1 ? int(cluster_rank()) : 0;
+  const int tile = blockIdx.x / splits;
+  const int f0 = (tile % f_tiles) * kOut, t0 = (tile / f_tiles) * BT;
+  const int k_tiles = (k + kBK - 1) / kBK;
+  const int per = (k_tiles + splits - 1) / splits;
+  const int kt0 = min(rank * per, k_tiles), kt1 = min(kt0 + per, k_tiles);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, C::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    bool ok = true;
+    for (int kt = kt0; kt < kt1; ++kt) {
+      const int it = kt - kt0, s = it % C::kStages;
+      if (it >= C::kStages) ok = lin_wait(&empty[s], (it / C::kStages - 1) & 1);
+      if (!ok) break;
+      uint8_t* st = smem + s * C::kStage;
+      mbar_expect_tx(&full[s], C::kStage);
+      load_features<kGated>(st, &maps.a_hi, &full[s], maps.a_kmajor, f0, e.feats, kt * kBK);
+      if constexpr (C::kAParts == 2)
+        load_features<kGated>(st + kABytes, &maps.a_lo, &full[s], maps.a_kmajor, f0, e.feats,
+                              kt * kBK);
+      uint8_t* sb = st + kABytes * C::kAParts;
+      load_rows<BT>(sb, &maps.b_hi, &full[s], maps.b_kmajor, t0, kt * kBK);
+      if constexpr (C::kBParts == 2)
+        load_rows<BT>(sb + C::kBBytes, &maps.b_lo, &full[s], maps.b_kmajor, t0, kt * kBK);
+    }
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t idesc = lin_idesc(128, BT, !maps.a_kmajor, !maps.b_kmajor);
+    bool ok = true;
+    for (int kt = kt0; kt < kt1; ++kt) {
+      const int it = kt - kt0, s = it % C::kStages;
+      ok = lin_wait(&full[s], (it / C::kStages) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t a_hi = smem_u32(smem + s * C::kStage);
+      const uint32_t b_hi = a_hi + kABytes * C::kAParts;
+#pragma unroll
+      for (int ks = 0; ks < kBK / 16; ++ks) {
+        const uint64_t dah = lin_desc(a_hi, maps.a_kmajor, ks);
+        const uint64_t dbh = lin_desc(b_hi, maps.b_kmajor, ks);
+        umma_bf16(tmem, dah, dbh, idesc, (it > 0 || ks > 0) ? 1u : 0u);
+        if constexpr (PREC == 3)
+          umma_bf16(tmem, lin_desc(a_hi + kABytes, maps.a_kmajor, ks), dbh, idesc, 1u);
+        if constexpr (PREC >= 2)
+          umma_bf16(tmem, dah, lin_desc(b_hi + C::kBBytes, maps.b_kmajor, ks), idesc, 1u);
+      }
+      umma_commit(&empty[s]);
+    }
+    umma_commit(done);
+  }
+  __syncwarp();
+  // every MMA of this CTA has completed: the accumulator may be read, and the
+  // stages hold nothing that is still needed
+  const bool ok = lin_wait(done, 0) && *reinterpret_cast<volatile int*>(&g_linear_status) == 0;
+  tc_fence_after();
+  float* partial = reinterpret_cast<float*>(smem);  // [token][lane]
+  const int toks = min(BT, e.toks - t0);
+  if (warp >= 2 && warp < 6 && __all_sync(0xffffffffu, ok)) {
+    const int quarter = warp & 3;
+    const int f = quarter * 32 + lane;
+    constexpr int kCols = BT < 32 ? 32 : BT;
+#pragma unroll 1
+    for (int col = 0; col < kCols && col < toks; col += 32) {
+      float v[32];
+      tmem_ld32(tmem + (uint32_t(quarter * 32) << 16) + col, v);
+#pragma unroll
+      for (int q = 0; q < 32; ++q)
+        if (col + q < toks) partial[(col + q) * kTileF + f] = kt1 > kt0 ? v[q] : 0.f;
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (splits > 1) cluster_sync_all(); else __syncthreads();
+  if (ok) {
+    const int share = (toks + splits - 1) / splits;
+    const int first = rank * share, last = min(first + share, toks);
+    const int f = threadIdx.x % kOut;
+    const uint32_t base = smem_u32(partial);
+    if (f0 + f < e.feats) {
+      for (int t = first + int(threadIdx.x) / kOut; t < last; t += kSplitThreads / kOut) {
+        float z = 0.f, zu = 0.f;
+        if (splits == 1) {
+          z = partial[t * kTileF + f];
+          if (kGated) zu = partial[t * kTileF + kOut + f];
+        } else {
+          for (int s = 0; s < splits; ++s) {
+            const uint32_t at = map_rank(base + uint32_t(t * kTileF + f) * 4u, s);
+            z += ld_cluster(at);
+            if (kGated) zu += ld_cluster(at + kOut * 4u);
+          }
+        }
+        finish<kGated>(e, f0 + f, t0 + t, z, zu);
+      }
+    }
+  }
+  if (!ok) {  // let issued copies land before the CTA exits
+    const uint64_t t = globaltimer();
+    while (globaltimer() - t < 1000000ull) {
+    }
+  }
+  // no CTA leaves while another may still read its partial tile
+  __syncwarp();
+  if (splits > 1) cluster_sync_all(); else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+// 3-D tiled bf16 map of an operand: K-major boxes {64 k, box_rows}, MN-major
+// boxes {64 columns, 64 k}; 128-byte swizzle.
+bool lin_map(CUtensorMap* map, const void* p, bool kmajor, int64_t rows, int64_t k, int64_t ld,
+             int box_rows) {
+  EncodeTiledFn encode = encode_fn();
+  if (!encode) return false;
+  const int64_t inner = kmajor ? k : rows, outer = kmajor ? rows : k;
+  const cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(outer), 1};
+  const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, cuuint64_t(ld) * 2 * cuuint64_t(outer)};
+  const cuuint32_t box[3] = {64, cuuint32_t(kmajor ? box_rows : kBK), 1};
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box,
+                elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename Kernel>
+int raise_smem(Kernel kernel, int bytes, std::atomic<bool>* configured) {
+  const int dev = current_device();
+  if (dev < 0) return MR_ERR_DEVICE;
+  if (configured[dev].load(std::memory_order_acquire)) return MR_OK;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return MR_ERR_LAUNCH;
+  }
+  configured[dev].store(true, std::memory_order_release);
+  return MR_OK;
+}
+
+template <int BT, int PREC, bool kGated>
+int launch_split(const LinMaps& maps, const LinEpilogue& e, int k, int splits, int64_t f_tiles,
+                 int64_t t_tiles, cudaStream_t stream) {
+  using C = SplitCfg<BT, PREC>;
+  static std::atomic<bool> configured[kMaxDevices];
+  auto kernel = linear_split_kernel<BT, PREC, kGated>;
+  const int st = raise_smem(kernel, C::kSmem, configured);
+  if (st != MR_OK) return st;
+  const int64_t grid = f_tiles * t_tiles * splits;
+  if (grid > 0x7fffffff) return MR_ERR_ARGUMENT;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(splits);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, maps, e, k, splits, int(f_tiles));
+  if (err != cudaSuccess) {
+    set_cuda_error(err);
+    cudaGetLastError();
+    return MR_ERR_LAUNCH;
+  }
+  return launch_status();
+}
+
+struct LinPlan {
+  int bt, splits;
+};
+
+// Token tile: the smallest that holds the tokens, up to 128.  K is divided so
+// that about two CTAs per SM are at work, each with at least four K slices.
+LinPlan plan_linear(int64_t f_tiles, int64_t toks, int64_t k, int b_kmajor, int splits) {
+  LinPlan p;
+  p.bt = toks <= 16 ? 16 : toks <= 32 ? 32 : toks <= 64 ? 64 : 128;
+  if (!b_kmajor && p.bt < 64) p.bt = 64;  // MN-major boxes are 64 tokens wide
+  const int64_t tiles = f_tiles * ((toks + p.bt - 1) / p.bt);
+  const int64_t k_tiles = (k + kBK - 1) / kBK;
+  p.splits = splits;
+  if (!splits) {
+    const int64_t at_once = int64_t(sm_count()) * (p.bt <= 64 ? 2 : 1);
+    p.splits = 1;
+    while (p.splits < 8 && tiles * p.splits * 2 <= at_once && k_tiles / (p.splits * 2) >= 4)
+      p.splits *= 2;
+  }
+  return p;
+}
+
+template <int PREC, bool kGated>
+int run_linear(LinMaps& maps, const LinEpilogue& e, const void* a_hi, const void* a_lo, int64_t lda,
+               const void* b_hi, const void* b_lo, int64_t ldb, int64_t rows_a, int64_t k,
+               int splits, cudaStream_t stream) {
+  constexpr int kOut = kGated ? kTileF / 2 : kTileF;
+  const int64_t f_tiles = (int64_t(e.feats) + kOut - 1) / kOut;
+  const LinPlan p = plan_linear(f_tiles, e.toks, k, maps.b_kmajor, splits);
+  const bool good =
+      lin_map(&maps.a_hi, a_hi, maps.a_kmajor, rows_a, k, lda, kOut) &&
+      lin_map(&maps.b_hi, b_hi, maps.b_kmajor, e.toks, k, ldb, p.bt) &&
+      (PREC < 3 || lin_map(&maps.a_lo, a_lo, maps.a_kmajor, rows_a, k, lda, kOut)) &&
+      (PREC < 2 || lin_map(&maps.b_lo, b_lo, maps.b_kmajor, e.toks, k, ldb, p.bt));
+  if (!good) return MR_ERR_ALIGNMENT;
+  const int64_t t_tiles = (int64_t(e.toks) + p.bt - 1) / p.bt;
+  switch (p.bt) {
+    case 16: return launch_split<16, PREC, kGated>(maps, e, int(k), p.splits, f_tiles, t_tiles, stream);
+    case 32: return launch_split<32, PREC, kGated>(maps, e, int(k), p.splits, f_tiles, t_tiles, stream);
+    case 64: return launch_split<64, PREC, kGated>(maps, e, int(k), p.splits, f_tiles, t_tiles, stream);
+    default: return launch_split<128, PREC, kGated>(maps, e, int(k), p.splits, f_tiles, t_tiles, stream);
+  }
+}
+
+}  // namespace
+
+int linear_status(int reset) {
+  int v = 0;
+  const cudaError_t e = cudaMemcpyFromSymbol(&v, g_linear_status, sizeof(int));
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return MR_ERR_LAUNCH;
+  }
+  if (reset && v) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace mr
+
+using namespace mr;
+
+extern "C" int mr_linear(const mr_linear_operand* x, const mr_linear_operand* w, int64_t toks,
+                         int64_t feats, int64_t k, int act, const float* bias,
+                         const void* residual, int residual_dtype, int64_t ldr, void* out,
+                         int out_dtype, uint16_t* out_lo, float* out_t32, int64_t ldo, float* pre,
+                         int64_t ldp, int splits, void* stream) {
+  if (!x || !w || !x->hi || !w->hi || !out || toks <= 0 || feats <= 0 || k <= 0)
+    return MR_ERR_ARGUMENT;
+  const int64_t most = 0x7fffff00;  // tile origins stay 32-bit
+  if (toks > most || feats > most / 2 || k > most || act < MR_ACT_NONE || act > MR_ACT_SWIGLU)
+    return MR_ERR_ARGUMENT;
+  if (splits != 0 && splits != 1 && splits != 2 && splits != 4 && splits != 8)
+    return MR_ERR_ARGUMENT;
+  const bool gated = act == MR_ACT_SWIGLU;
+  if ((gated && !w->kmajor) || (w->lo && !x->lo)) return MR_ERR_ARGUMENT;
+  if ((out_dtype != MR_F32 && out_dtype != MR_BF16) || (out_lo && out_dtype != MR_BF16) ||
+      (residual && residual_dtype != MR_F32 && residual_dtype != MR_BF16))
+    return MR_ERR_ARGUMENT;
+  const int64_t rows_w = gated ? 2 * feats : feats;
+  if ((x->kmajor ? x->ld < k : x->ld < toks) || (w->kmajor ? w->ld < k : w->ld < rows_w) ||
+      ldo < feats || (residual && ldr < feats) || (pre && ldp < rows_w))
+    return MR_ERR_ARGUMENT;
+  if (!aligned16(x->hi) || !aligned16(x->lo) || !aligned16(w->hi) || !aligned16(w->lo) ||
+      x->ld % 8 || w->ld % 8)
+    return MR_ERR_ALIGNMENT;
+  LinMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  maps.a_kmajor = w->kmajor != 0;
+  maps.b_kmajor = x->kmajor != 0;
+  LinEpilogue e;
+  e.bias = bias;
+  e.residual = residual;
+  e.out = out;
+  e.lo = out_lo;
+  e.t32 = out_t32;
+  e.pre = pre;
+  e.ldr = ldr;
+  e.ldo = ldo;
+  e.ldp = ldp;
+  e.residual_dtype = residual_dtype;
+  e.out_dtype = out_dtype;
+  e.act = act;
+  e.feats = int(feats);
+  e.toks = int(toks);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define MR_LINEAR(PREC)                                                                        \
+  (gated ? run_linear<PREC, true>(maps, e, w->hi, w->lo, w->ld, x->hi, x->lo, x->ld, rows_w, k, \
+                                  splits, st)                                                  \
+         : run_linear<PREC, false>(maps, e, w->hi, w->lo, w->ld, x->hi, x->lo, x->ld, rows_w, k, \
+                                   splits, st))
+  if (w->lo) return MR_LINEAR(3);
+  if (x->lo) return MR_LINEAR(2);
+  return MR_LINEAR(1);
+#undef MR_LINEAR
+}

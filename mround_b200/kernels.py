@@ -23,6 +23,8 @@ __all__ = [
     "gemm",
     "gemm_batched",
     "gemm_tf32",
+    "linear",
+    "linear_bwd",
     "loss_apply",
     "loss_hist_pass",
     "loss_outlier",
@@ -990,3 +992,184 @@ def distill_topk_grad(logits, t_logits, t_index, *, temperature: float = 1.0, we
     _, _, ldg = _logit_rows(out)
     _distill(logits, t_logits, t_index, temperature, weight, loss, out, (None, None), ldg)
     return loss, out
+
+
+ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "swiglu": 4}
+LINEAR_SPLITS = (1, 2, 4, 8)
+
+
+def _act_code(act: str) -> int:
+    code = ACTIVATIONS.get(act)
+    if code is None:
+        raise SchemeError(f"act must be one of {', '.join(ACTIVATIONS)}, got {act!r}")
+    return code
+
+
+def _parts(t, name: str):
+    """(hi, lo or None) of a bf16 operand given as a tensor or as a pair."""
+    hi, lo = t if isinstance(t, (tuple, list)) else (t, None)
+    for part in (hi, lo):
+        if part is None and part is lo:
+            continue
+        if part.dim() != 2 or part.dtype != torch.bfloat16:
+            raise SchemeError(f"{name} must be a 2-D bfloat16 tensor or a (hi, lo) pair of them")
+        if part.shape != hi.shape or part.stride() != hi.stride():
+            raise SchemeError(f"{name}'s parts must have one shape and layout")
+    return hi, lo
+
+
+def _operand(parts, name: str, kmajor: bool):
+    """``mr_linear_operand`` of parts whose columns (K-major) or rows are k."""
+    from mround_b200._native import LinearOperand
+
+    hi, lo = parts
+    rows, cols = hi.shape
+    ld = hi.stride(0) if rows > 1 else -(-cols // 8) * 8
+    if (cols > 1 and hi.stride(1) != 1) or ld < cols or ld % 8:
+        raise SchemeError(f"{name} needs contiguous columns and a row stride that is a multiple "
+                          f"of 8, got strides {hi.stride()}")
+    return LinearOperand(hi.data_ptr(), None if lo is None else lo.data_ptr(), ld, int(kmajor))
+
+
+def _row_stride(t, rows: int, cols: int, dtypes, name: str) -> int:
+    if t.dtype not in dtypes or t.shape != (rows, cols):
+        raise SchemeError(f"{name} must be ({rows}, {cols}) of {dtypes}, got {tuple(t.shape)} "
+                          f"{t.dtype}")
+    ld = t.stride(0) if rows > 1 else cols
+    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+        raise SchemeError(f"{name} needs contiguous columns in rows that do not overlap")
+    return ld
+
+
+_LINEAR_OUT = (torch.float32, torch.bfloat16)
+
+
+def _linear_call(dev, x, w, toks, feats, k, act, bias, residual, ldr, out, lo, t32, ldo, pre, ldp,
+                 splits):
+    timing = GEMM_EVENTS is not None
+    if timing:
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    _launch("mr_linear", dev, _ref(x), _ref(w), toks, feats, k, act, ptr(bias), ptr(residual),
+            0 if residual is None else DTYPES[residual.dtype], ldr, out.data_ptr(),
+            DTYPES[out.dtype], ptr(lo), ptr(t32), ldo, ptr(pre), ldp, splits)
+    if timing:
+        end.record()
+        products = 1 + (x.lo is not None) + (w.lo is not None)
+        GEMM_EVENTS.append((start, end, 2.0 * toks * feats * (2 if act == 4 else 1) * k, products))
+
+
+def linear(x, w, *, bias=None, act: str = "none", residual=None, out=None, dtype=None,
+           split: bool = False, t32=None, pre=None, splits: int | None = None):
+    """K13: ``act(x @ w.T + bias) + residual`` in one kernel, float32 accumulation.
+
+    ``x`` (T, k) and ``w`` (features, k): bfloat16 tensors with contiguous
+    columns and a row stride that is a multiple of 8, or (hi, lo) pairs of them
+    as :func:`split_bf16` makes (``w`` a pair only with ``x`` a pair).
+    ``act``: "none", "silu", "gelu" (erf), "gelu_tanh" or "swiglu", where ``w``
+    holds [gate | up] rows and the output has half as many columns.  ``bias``
+    float32 (features,); ``residual`` float32 or bfloat16 of the output's shape.
+
+    The output is ``dtype`` (float32 or bfloat16; by default bfloat16, float32
+    when ``x`` is a pair), in ``out`` when given (which may be ``residual``),
+    or with ``split`` a bf16 (hi, lo) pair.  ``t32``: a contiguous float32
+    tensor that also receives the output rounded to tf32.  ``pre``: a float32
+    (T, features) tensor that receives ``x @ w.T + bias``, for
+    :func:`linear_bwd`.
+
+    ``splits``: how many CTAs share the k of one output tile (1, 2, 4 or 8),
+    chosen by size when None.  It fixes the order of the sums: with 1 a token's
+    result is the same whatever other tokens are in the call."""
+    code = _act_code(act)
+    xp, wp = _parts(x, "x"), _parts(w, "w")
+    dev = _device_of(x=xp[0], x_lo=xp[1], w=wp[0], w_lo=wp[1], bias=bias, residual=residual,
+                     out=out, t32=t32, pre=pre)
+    toks, k = xp[0].shape
+    rows = wp[0].shape[0]
+    if wp[0].shape[1] != k or k == 0 or rows == 0:
+        raise SchemeError(f"x {tuple(xp[0].shape)} and w {tuple(wp[0].shape)} do not share a k")
+    if wp[1] is not None and xp[1] is None:
+        raise SchemeError("w is a (hi, lo) pair but x is not")
+    if act == "swiglu" and rows % 2:
+        raise SchemeError(f"a swiglu weight has as many gate as up rows, got {rows} rows")
+    if splits is not None and splits not in LINEAR_SPLITS:
+        raise SchemeError(f"splits must be one of {LINEAR_SPLITS}, got {splits}")
+    feats = rows // 2 if act == "swiglu" else rows
+    lo = None
+    if split:
+        if out is not None or dtype is not None:
+            raise SchemeError("a split output is allocated by the call")
+        out, lo = _pair((toks, feats), dev)
+    elif out is None:
+        out = torch.empty((toks, feats), device=dev,
+                          dtype=dtype or (torch.bfloat16 if xp[1] is None else torch.float32))
+    elif dtype is not None and out.dtype != dtype:
+        raise SchemeError(f"out is {out.dtype}, not {dtype}")
+    ldo = _row_stride(out, toks, feats, _LINEAR_OUT, "out")
+    if t32 is not None:
+        if _row_stride(t32, toks, feats, (torch.float32,), "t32") != ldo:
+            raise SchemeError("t32 must have the output's row stride")
+    ldr = 0 if residual is None else _row_stride(residual, toks, feats, _LINEAR_OUT, "residual")
+    ldp = 0 if pre is None else _row_stride(pre, toks, rows, (torch.float32,), "pre")
+    if bias is not None:
+        _ptr(bias, torch.float32, "bias", rows)
+    if toks:
+        _linear_call(dev, _operand(xp, "x", True), _operand(wp, "w", True), toks, feats, k, code,
+                     bias, residual, ldr, out, lo, t32, ldo, pre, ldp, splits or 0)
+    return (out, lo) if split else out
+
+
+def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False, dtype=None,
+               splits: int | None = None):
+    """Gradients of :func:`linear`: ``(dx, dw, dbias or None)`` from ``dy``
+    (float32 or bfloat16), the operands and the ``pre`` that the forward wrote
+    (not needed where ``act`` is "none").  The residual's gradient is ``dy``.
+
+    ``dz = dy * act'(pre)`` is carried as a bf16 pair; ``dx = dz @ w`` and
+    ``dw = dz.T @ x`` are ``dtype`` (float32 or bfloat16; by default as the
+    output of :func:`linear`), the bias gradient float32."""
+    code = _act_code(act)
+    xp, wp = _parts(x, "x"), _parts(w, "w")
+    dev = _device_of(dy=dy, x=xp[0], x_lo=xp[1], w=wp[0], w_lo=wp[1], pre=pre)
+    toks, k = xp[0].shape
+    rows = wp[0].shape[0]
+    if wp[0].shape[1] != k or k == 0 or rows == 0 or (act == "swiglu" and rows % 2):
+        raise SchemeError(f"x {tuple(xp[0].shape)} and w {tuple(wp[0].shape)} are not the operands "
+                          "of a linear")
+    feats = rows // 2 if act == "swiglu" else rows
+    ldy = _row_stride(dy, toks, feats, _LINEAR_OUT, "dy")
+    if pre is None and act != "none":
+        raise SchemeError(f"the gradient of {act} needs the pre-activation")
+    ldp = 0 if pre is None else _row_stride(pre, toks, rows, (torch.float32,), "pre")
+    if splits is not None and splits not in LINEAR_SPLITS:
+        raise SchemeError(f"splits must be one of {LINEAR_SPLITS}, got {splits}")
+    out_dtype = dtype or (torch.bfloat16 if xp[1] is None else torch.float32)
+    if out_dtype not in _LINEAR_OUT:
+        raise SchemeError(f"dtype must be float32 or bfloat16, got {out_dtype}")
+    x_op, w_op = _operand(xp, "x", False), _operand(wp, "w", False)
+    dx = torch.empty((toks, k), dtype=out_dtype, device=dev)
+    dw = torch.empty((rows, k), dtype=out_dtype, device=dev)
+    db = torch.empty(rows, dtype=torch.float32, device=dev) if bias_grad else None
+    if toks == 0:
+        dw.zero_()
+        if db is not None:
+            db.zero_()
+        return dx, dw, db
+    ldz = -(-rows // 8) * 8
+    hi, lo = _pair((toks, ldz), dev)
+    scratch = None
+    if bias_grad:
+        nbytes = int(lib().mr_act_grad_workspace_bytes(toks, feats, code))
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    z = None if act == "none" else pre.data_ptr()
+    _launch("mr_act_grad", dev, dy.data_ptr(), DTYPES[dy.dtype], ldy, z, ldp, toks, feats, code,
+            hi.data_ptr(), lo.data_ptr(), ldz, None if db is None else db.data_ptr(),
+            None if scratch is None else scratch.data_ptr())
+    n = splits or 0
+    dz = (hi[:, :rows], lo[:, :rows])
+    _linear_call(dev, _operand(dz, "dz", True), w_op, toks, k, rows, 0, None, None, 0, dx, None,
+                 None, k, None, 0, n)
+    _linear_call(dev, _operand(dz, "dz", False), x_op, rows, k, toks, 0, None, None, 0, dw, None,
+                 None, k, None, 0, n)
+    return dx, dw, db
