@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(kSplitThreads)
 #pragma unroll 1
     for (int col = 0; col < kCols && col < toks; col += 32) {
       float v[32];
+      __syncwarp();
       tmem_ld32(tmem + (uint32_t(quarter * 32) << 16) + col, v);
 #pragma unroll
       for (int q = 0; q < 32; ++q)
@@ -331,6 +332,382 @@ __global__ void __launch_bounds__(kSplitThreads)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+
+// ---------------------------------------------------------------- wide kernel
+// Many tokens: a persistent kernel of CTA pairs.  A pair computes 256 features
+// x 256 tokens with tcgen05.mma.cta_group::2 (M = 256, N = 256): each CTA
+// stages its 128 feature rows and half of the token rows and keeps its 128
+// lanes x 256 columns of the accumulator, so a stage holds 256 rows of k for
+// 2 x 128 x 256 flops per k and CTA -- a third less than a 128 x 256 tile of
+// one CTA.  Two accumulators: the epilogue of one tile overlaps the MMAs of
+// the next.
+//
+// The leader (rank 0) issues the MMAs for both.  Both CTAs' loads complete on
+// the leader's "full" barrier; the MMAs' commits free the stage, and publish
+// the accumulator, on the barriers of both; the epilogue warps of both arrive
+// on the leader's "tmem_empty".
+constexpr int kWideThreads = 192;
+constexpr int kWideT = 256;          // tokens per tile
+constexpr int kWideBufs = 2;         // accumulators of 256 columns
+
+template <int PREC>
+struct WideCfg {
+  static constexpr int kAParts = PREC == 3 ? 2 : 1;
+  static constexpr int kBParts = PREC >= 2 ? 2 : 1;
+  static constexpr int kBBytes = kWideT / 2 * kBK * 2;
+  static constexpr int kStage = kABytes * kAParts + kBBytes * kBParts;
+  static constexpr int kStages = 192 * 1024 / kStage;
+  // SwiGLU: two buffers of 32 x 32 float32 in each direction per pair of warps
+  static constexpr int kExchange = 2 * 2 * 2 * 32 * 32 * 4;
+  static constexpr int kSmem = kStages * kStage + kExchange + 1024 /* align */ + 256;
+  static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
+};
+
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar,
+                                              int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(0)
+      : "memory");
+}
+
+// One operand part of ROWS rows (features or tokens) of a stage.
+template <int ROWS>
+__device__ __forceinline__ void load_pair_rows(uint8_t* dst, const CUtensorMap* map, uint32_t bar,
+                                               bool kmajor, int row0, int k0) {
+  if (kmajor) {
+    tma_load_pair(dst, map, bar, k0, row0);
+  } else {
+#pragma unroll
+    for (int c = 0; c < ROWS / 64; ++c)
+      tma_load_pair(dst + c * 64 * kBK * 2, map, bar, row0 + c * 64, k0);
+  }
+}
+
+template <bool kGated>
+__device__ __forceinline__ void load_pair_features(uint8_t* dst, const CUtensorMap* map,
+                                                   uint32_t bar, bool kmajor, int f0, int up0,
+                                                   int k0) {
+  if constexpr (kGated) {
+    tma_load_pair(dst, map, bar, k0, f0);
+    tma_load_pair(dst + kABytes / 2, map, bar, k0, up0 + f0);
+  } else {
+    load_pair_rows<kTileF>(dst, map, bar, kmajor, f0, k0);
+  }
+}
+
+__device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+
+// Arrives on the barrier at this offset in both CTAs once the MMAs so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Whether `ok` holds in all four epilogue warps.
+__device__ __forceinline__ bool epilogue_agrees(bool ok) {
+  int all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.s32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred.aligned q, 3, 128, p;\n\t"
+      "selp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(int(ok))
+      : "memory");
+  return all != 0;
+}
+
+// Tiles in groups of 8 token tiles that sweep the features together, so that
+// the tiles in flight share their operands in L2.
+__device__ __forceinline__ void wide_tile(int t, int f_tiles, int t_tiles, int* ft, int* tt) {
+  constexpr int G = 8;
+  const int group = t / (G * f_tiles);
+  const int first = group * G;
+  const int rows = min(G, t_tiles - first);
+  const int r = t - first * f_tiles;
+  *tt = first + r % rows;
+  *ft = r / rows;
+}
+
+// The epilogue of 32 tokens of one feature (lane): v holds z without bias.
+template <bool kGated>
+__device__ __forceinline__ void finish32(const LinEpilogue& e, int f, int t0, float (&v)[32],
+                                         const float (&up)[32]) {
+  const int n = min(32, e.toks - t0);
+  if (f >= e.feats) return;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = kGated ? silu1(v[i]) * up[i] : v[i];
+  if (!kGated && e.act != MR_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = act1(v[i], e.act);
+  }
+  if (e.residual) {
+    float r[32];
+    if (e.residual_dtype == MR_F32) {
+      const float* p = static_cast<const float*>(e.residual) + int64_t(t0) * e.ldr + f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = i < n ? p[i * e.ldr] : 0.f;
+    } else {
+      const uint16_t* p = static_cast<const uint16_t*>(e.residual) + int64_t(t0) * e.ldr + f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = i < n ? bf16_to_f32(p[i * e.ldr]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] += r[i];
+  }
+  const int64_t at = int64_t(t0) * e.ldo + f;
+  if (e.out_dtype == MR_F32) {
+    float* p = static_cast<float*>(e.out) + at;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) p[i * e.ldo] = v[i];
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(e.out) + at;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) p[i * e.ldo] = f32_to_bf16(v[i]);
+    if (e.lo) {
+      uint16_t* l = e.lo + at;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < n) l[i * e.ldo] = f32_to_bf16(__fsub_rn(v[i], bf16_to_f32(f32_to_bf16(v[i]))));
+    }
+  }
+  if (e.t32) {
+    float* p = e.t32 + at;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) p[i * e.ldo] = tf32_rna(v[i]);
+  }
+}
+
+// Stores 32 tokens of z for one feature (row of w).
+__device__ __forceinline__ void store_pre(const LinEpilogue& e, int row, bool on, int t0,
+                                          const float (&v)[32]) {
+  const int n = min(32, e.toks - t0);
+  if (!on) return;
+  float* p = e.pre + int64_t(t0) * e.ldp + row;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (i < n) p[i * e.ldp] = v[i];
+}
+
+template <int PREC, bool kGated>
+__global__ void __launch_bounds__(kWideThreads, 1) __cluster_dims__(2, 1, 1)
+    linear_wide_kernel(const __grid_constant__ LinMaps maps,
+                       const __grid_constant__ LinEpilogue e, int k, int f_tiles, int t_tiles) {
+  using C = WideCfg<PREC>;
+  constexpr int kOut = kGated ? kTileF / 2 : kTileF;  // outputs per CTA
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  float* exchange = reinterpret_cast<float*>(smem + C::kStages * C::kStage);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStage + C::kExchange);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* tmem_full = empty + C::kStages;        // [kWideBufs]
+  uint64_t* tmem_empty = tmem_full + kWideBufs;    // [kWideBufs], the leader's are used
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + kWideBufs);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(cluster_rank());
+  const int pairs = gridDim.x / 2, first = blockIdx.x / 2;
+  const int k_tiles = (k + kBK - 1) / kBK;
+  const int total = f_tiles * t_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < kWideBufs; ++b) {
+      mbar_init(&tmem_full[b], 1);
+      mbar_init(&tmem_empty[b], 8);  // four epilogue warps of each CTA
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  cluster_sync_all();  // both CTAs' barriers exist before either signals the other's
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (int t = first; t < total && ok; t += pairs) {
+        int ft, tt;
+        wide_tile(t, f_tiles, t_tiles, &ft, &tt);
+        const int f0 = (ft * 2 + rank) * kOut, t0 = tt * kWideT + rank * (kWideT / 2);
+        for (int kt = 0; kt < k_tiles; ++kt, ++it) {
+          const int s = it % C::kStages;
+          if (it >= C::kStages) ok = lin_wait(&empty[s], (it / C::kStages - 1) & 1);
+          if (!ok) break;
+          uint8_t* st = smem + s * C::kStage;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * C::kStage);
+          const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
+          load_pair_features<kGated>(st, &maps.a_hi, bar, maps.a_kmajor, f0, e.feats, kt * kBK);
+          if constexpr (C::kAParts == 2)
+            load_pair_features<kGated>(st + kABytes, &maps.a_lo, bar, maps.a_kmajor, f0, e.feats,
+                                       kt * kBK);
+          uint8_t* sb = st + kABytes * C::kAParts;
+          load_pair_rows<kWideT / 2>(sb, &maps.b_hi, bar, maps.b_kmajor, t0, kt * kBK);
+          if constexpr (C::kBParts == 2)
+            load_pair_rows<kWideT / 2>(sb + C::kBBytes, &maps.b_lo, bar, maps.b_kmajor, t0,
+                                       kt * kBK);
+        }
+      }
+      // the last use of every stage has been signalled before this CTA leaves
+      for (int i = max(0, it - C::kStages); i < it && ok; ++i)
+        ok = lin_wait(&empty[i % C::kStages], (i / C::kStages) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = lin_idesc(256, kWideT, !maps.a_kmajor, !maps.b_kmajor);
+      int it = 0, j = 0;
+      for (int t = first; t < total && ok; t += pairs, ++j) {
+        const int b = j % kWideBufs;
+        if (j >= kWideBufs) ok = lin_wait(&tmem_empty[b], (j / kWideBufs - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + uint32_t(b * kWideT);
+        for (int kt = 0; kt < k_tiles; ++kt, ++it) {
+          const int s = it % C::kStages;
+          ok = lin_wait(&full[s], (it / C::kStages) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_hi = smem_u32(smem + s * C::kStage);
+          const uint32_t b_hi = a_hi + kABytes * C::kAParts;
+#pragma unroll
+          for (int ks = 0; ks < kBK / 16; ++ks) {
+            const uint64_t dah = lin_desc(a_hi, maps.a_kmajor, ks);
+            const uint64_t dbh = lin_desc(b_hi, maps.b_kmajor, ks);
+            umma_pair(d, dah, dbh, idesc, (kt > 0 || ks > 0) ? 1u : 0u);
+            if constexpr (PREC == 3)
+              umma_pair(d, lin_desc(a_hi + kABytes, maps.a_kmajor, ks), dbh, idesc, 1u);
+            if constexpr (PREC >= 2)
+              umma_pair(d, dah, lin_desc(b_hi + C::kBBytes, maps.b_kmajor, ks), idesc, 1u);
+          }
+          commit_pair(&empty[s]);
+        }
+        if (!ok) break;
+        commit_pair(&tmem_full[b]);
+      }
+    }
+  } else {
+    const int quarter = warp & 3;  // lanes 32 quarter .. + 31
+    const int l = quarter * 32 + lane;
+    const int half = quarter >> 1, pair = quarter & 1;  // SwiGLU: gate (0) or up (1) rows
+    const uint32_t empty_at = map_rank(smem_u32(tmem_empty), 0);
+    int j = 0;
+    for (int t = first; t < total; t += pairs, ++j) {
+      int ft, tt;
+      wide_tile(t, f_tiles, t_tiles, &ft, &tt);
+      const int b = j % kWideBufs;
+      ok = lin_wait(&tmem_full[b], (j / kWideBufs) & 1) &&
+           *reinterpret_cast<volatile int*>(&g_linear_status) == 0;
+      tc_fence_after();
+      __syncwarp();
+      // the four warps go on, or give up, together: they wait for one another below
+      ok = epilogue_agrees(ok);
+      if (!ok) break;
+      const int f0 = (ft * 2 + rank) * kOut, t0 = tt * kWideT;
+      const uint32_t lanes = tmem + uint32_t(b * kWideT) + (uint32_t(quarter * 32) << 16);
+      const int f = f0 + (kGated ? l % kOut : l);
+      const int row = kGated ? f + half * e.feats : f;  // row of w
+      const bool on = f < e.feats;
+      const float bias = e.bias && on ? e.bias[row] : 0.f;
+      if constexpr (!kGated) {
+#pragma unroll 1
+        for (int col = 0; col < kWideT && t0 + col < e.toks; col += 32) {
+          float v[32];
+          __syncwarp();
+          tmem_ld32(lanes + col, v);
+          if (e.bias) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += bias;
+          }
+          if (e.pre) store_pre(e, row, on, t0 + col, v);
+          finish32<false>(e, f, t0 + col, v, v);
+        }
+      } else {
+        // warps q (gate) and q + 2 (up) hold the same features: of every 64
+        // tokens the gate warp finishes the first 32, the up warp the others
+#pragma unroll 1
+        for (int col = 0; col < kWideT; col += 64) {
+          float mine[32], give[32];
+          __syncwarp();
+          tmem_ld32(lanes + col + half * 32, mine);
+          tmem_ld32(lanes + col + (1 - half) * 32, give);
+          if (e.bias) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              mine[i] += bias;
+              give[i] += bias;
+            }
+          }
+          const int mine0 = t0 + col + half * 32, give0 = t0 + col + (1 - half) * 32;
+          if (e.pre) {
+            store_pre(e, row, on, mine0, mine);
+            store_pre(e, row, on, give0, give);
+          }
+          float* box = exchange + ((col >> 6) & 1) * 4096 + pair * 2048;
+          float* to = box + (1 - half) * 1024;
+          float* from = box + half * 1024;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) to[i * 32 + lane] = give[i];
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
+          float other[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) other[i] = from[i * 32 + lane];
+          if (half == 0)
+            finish32<true>(e, f, mine0, mine, other);
+          else
+            finish32<true>(e, f, mine0, other, mine);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_remote(empty_at + uint32_t(b) * 8u);
+    }
+  }
+  if (!ok) {  // let issued copies land before the CTA exits
+    const uint64_t t = globaltimer();
+    while (globaltimer() - t < 1000000ull) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
 }
 
@@ -398,14 +775,30 @@ int launch_split(const LinMaps& maps, const LinEpilogue& e, int k, int splits, i
   return launch_status();
 }
 
+template <int PREC, bool kGated>
+int launch_wide(const LinMaps& maps, const LinEpilogue& e, int k, int64_t f_tiles, int64_t t_tiles,
+                cudaStream_t stream) {
+  using C = WideCfg<PREC>;
+  static std::atomic<bool> configured[kMaxDevices];
+  auto kernel = linear_wide_kernel<PREC, kGated>;
+  const int st = raise_smem(kernel, C::kSmem, configured);
+  if (st != MR_OK) return st;
+  if (f_tiles * t_tiles > 0x7fffffff) return MR_ERR_ARGUMENT;
+  const int64_t pairs = sm_count() / 2;
+  const int64_t grid = 2 * (f_tiles * t_tiles < pairs ? f_tiles * t_tiles : pairs);
+  kernel<<<unsigned(grid), kWideThreads, C::kSmem, stream>>>(maps, e, k, int(f_tiles), int(t_tiles));
+  return launch_status();
+}
+
 struct LinPlan {
-  int bt, splits;
+  int bt, splits;  // bt = kWideT: the wide kernel
 };
 
 // Token tile: the smallest that holds the tokens, up to 128.  K is divided so
 // that about two CTAs per SM are at work, each with at least four K slices.
 LinPlan plan_linear(int64_t f_tiles, int64_t toks, int64_t k, int b_kmajor, int splits) {
   LinPlan p;
+  if (splits <= 1 && toks >= 512) return {kWideT, 1};
   p.bt = toks <= 16 ? 16 : toks <= 32 ? 32 : toks <= 64 ? 64 : 128;
   if (!b_kmajor && p.bt < 64) p.bt = 64;  // MN-major boxes are 64 tokens wide
   const int64_t tiles = f_tiles * ((toks + p.bt - 1) / p.bt);
@@ -427,12 +820,17 @@ int run_linear(LinMaps& maps, const LinEpilogue& e, const void* a_hi, const void
   constexpr int kOut = kGated ? kTileF / 2 : kTileF;
   const int64_t f_tiles = (int64_t(e.feats) + kOut - 1) / kOut;
   const LinPlan p = plan_linear(f_tiles, e.toks, k, maps.b_kmajor, splits);
+  const bool wide = p.bt == kWideT;
+  const int t_box = wide ? kWideT / 2 : p.bt;
   const bool good =
       lin_map(&maps.a_hi, a_hi, maps.a_kmajor, rows_a, k, lda, kOut) &&
-      lin_map(&maps.b_hi, b_hi, maps.b_kmajor, e.toks, k, ldb, p.bt) &&
+      lin_map(&maps.b_hi, b_hi, maps.b_kmajor, e.toks, k, ldb, t_box) &&
       (PREC < 3 || lin_map(&maps.a_lo, a_lo, maps.a_kmajor, rows_a, k, lda, kOut)) &&
-      (PREC < 2 || lin_map(&maps.b_lo, b_lo, maps.b_kmajor, e.toks, k, ldb, p.bt));
+      (PREC < 2 || lin_map(&maps.b_lo, b_lo, maps.b_kmajor, e.toks, k, ldb, t_box));
   if (!good) return MR_ERR_ALIGNMENT;
+  if (wide)
+    return launch_wide<PREC, kGated>(maps, e, int(k), (int64_t(e.feats) + 2 * kOut - 1) / (2 * kOut),
+                                     (int64_t(e.toks) + kWideT - 1) / kWideT, stream);
   const int64_t t_tiles = (int64_t(e.toks) + p.bt - 1) / p.bt;
   switch (p.bt) {
     case 16: return launch_split<16, PREC, kGated>(maps, e, int(k), p.splits, f_tiles, t_tiles, stream);
