@@ -729,21 +729,6 @@ bool lin_map(CUtensorMap* map, const void* p, bool kmajor, int64_t rows, int64_t
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename Kernel>
-int raise_smem(Kernel kernel, int bytes, std::atomic<bool>* configured) {
-  const int dev = current_device();
-  if (dev < 0) return MR_ERR_DEVICE;
-  if (configured[dev].load(std::memory_order_acquire)) return MR_OK;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    return MR_ERR_LAUNCH;
-  }
-  configured[dev].store(true, std::memory_order_release);
-  return MR_OK;
-}
-
 template <int BT, int PREC, bool kGated>
 int launch_split(const LinMaps& maps, const LinEpilogue& e, int k, int splits, int64_t f_tiles,
                  int64_t t_tiles, cudaStream_t stream) {

@@ -191,5 +191,21 @@ int sm_count() {
   return count;
 }
 
+// Raises a kernel's dynamic shared-memory limit once per device.
+template <typename Kernel>
+int raise_smem(Kernel kernel, int bytes, std::atomic<bool>* configured) {
+  const int dev = current_device();
+  if (dev < 0) return MR_ERR_DEVICE;
+  if (configured[dev].load(std::memory_order_acquire)) return MR_OK;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return MR_ERR_LAUNCH;
+  }
+  configured[dev].store(true, std::memory_order_release);
+  return MR_OK;
+}
+
 }  // namespace
 }  // namespace mr

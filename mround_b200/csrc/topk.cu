@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "rowtypes.cuh"
+#include "sm100.cuh"
 
 namespace mr {
 namespace {
@@ -240,12 +241,9 @@ __global__ void __launch_bounds__(kTopThreads, 3)
 template <typename T>
 int launch_topk(const void* logits, int64_t rows, int n, int64_t ld, int k, float* values,
                 int64_t* indices, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(
-      topk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(TopShared)));
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    return MR_ERR_LAUNCH;
-  }
+  static std::atomic<bool> configured[kMaxDevices];
+  const int status = raise_smem(topk_kernel<T>, int(sizeof(TopShared)), configured);
+  if (status != MR_OK) return status;
   int groups = 32;
   while (groups < k) groups *= 2;
   topk_kernel<T><<<unsigned(rows), kTopThreads, sizeof(TopShared), stream>>>(

@@ -775,31 +775,38 @@ def _interleaved(layout: str) -> int:
     return int(layout == "interleaved")
 
 
-def _device_of(**tensors) -> torch.device:
-    """The CUDA device all given tensors share."""
+def _device_of(names: str, *tensors) -> int:
+    """The index of the CUDA device all given tensors (None apart) share."""
     dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise PlatformError(f"{name} must be a CUDA tensor (there is no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise SchemeError(f"{name} is on {t.device}, expected {dev}")
+    for t in tensors:
+        if t is not None:
+            index = t.get_device()
+            if index != dev or index < 0:
+                if index < 0 or dev is not None:
+                    name = next(n for n, u in zip(names.split(), tensors) if u is t)
+                    if index < 0:
+                        raise PlatformError(f"{name} must be a CUDA tensor (there is no CPU "
+                                            "fallback)")
+                    raise SchemeError(f"{name} is on cuda:{index}, expected cuda:{dev}")
+                dev = index
     return dev
 
 
-def _launch(name: str, dev: torch.device, *args) -> None:
-    """One C entry point on ``dev``'s current stream (appended to ``args``)."""
+# the stream's handle alone: torch.cuda.current_stream() builds an object (3 us)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _launch(name: str, dev: int, *args) -> None:
+    """One C entry point on device ``dev``'s current stream (appended to ``args``)."""
     fn = getattr(lib(), name)
-    if dev.index == torch.cuda.current_device():
-        status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if dev == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, torch.cuda.current_stream().cuda_stream)
-    check(status, name)
-    _count()
+            status = fn(*args, _raw_stream(dev))
+    if status:
+        check(status, name)
+    LAUNCHES[0] += 1
 
 
 def _dtype_code(t: torch.Tensor, name: str) -> int:
@@ -817,10 +824,9 @@ def _rotary(q, k, cos, sin, positions, layout, out, transposed):
         raise SchemeError("q and k are (batch, positions, heads, head dim)")
     b, s, hq, d = q.shape
     if out is None:
-        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-               None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
+        out = (torch.empty_like(q), None if k is None else torch.empty_like(k))
     yq, yk = out
-    dev = _device_of(q=q, k=k, cos=cos, sin=sin, positions=positions, out_q=yq, out_k=yk)
+    dev = _device_of("q k cos sin positions out_q out_k", q, k, cos, sin, positions, yq, yk)
     code = _dtype_code(q, "q")
     if (k is None) != (yk is None):
         raise SchemeError("out is a (q, k) pair with k None exactly where k is")
@@ -916,13 +922,13 @@ def topk_logits(logits, k: int):
     ``logits``: (rows, vocabulary) float32, bfloat16 or float16, contiguous
     columns.  1 <= k <= min(vocabulary, 256).  Returns float32 values and int64
     columns, (rows, k) each -- what :func:`distill_topk` takes."""
-    dev = _device_of(logits=logits)
+    dev = _device_of("logits", logits)
     rows, n, ld = _logit_rows(logits)
     code = _dtype_code(logits, "logits")
     if not 1 <= k <= min(n, MAX_TOPK):
         raise SchemeError(f"k must be 1 to {min(n, MAX_TOPK)}, got {k}")
-    values = torch.empty((rows, k), dtype=torch.float32, device=dev)
-    index = torch.empty((rows, k), dtype=torch.int64, device=dev)
+    values = torch.empty((rows, k), dtype=torch.float32, device=logits.device)
+    index = torch.empty((rows, k), dtype=torch.int64, device=logits.device)
     if rows:
         _launch("mr_topk_logits", dev, logits.data_ptr(), rows, n, ld, k, code, values.data_ptr(),
                 index.data_ptr())
@@ -930,8 +936,7 @@ def topk_logits(logits, k: int):
 
 
 def _distill(logits, t_logits, t_index, temperature, weight, loss, grad, pair, ldg):
-    dev = _device_of(logits=logits, t_logits=t_logits, t_index=t_index, weight=weight, out=grad,
-                     out_hi=pair[0], out_lo=pair[1])
+    dev = _device_of("logits t_logits t_index weight out", logits, t_logits, t_index, weight, grad)
     rows, n, ld = _logit_rows(logits)
     code = _dtype_code(logits, "logits")
     if t_logits.dim() != 2 or t_logits.shape != t_index.shape or t_logits.shape[0] != rows:
@@ -1083,8 +1088,8 @@ def linear(x, w, *, bias=None, act: str = "none", residual=None, out=None, dtype
     result is the same whatever other tokens are in the call."""
     code = _act_code(act)
     xp, wp = _parts(x, "x"), _parts(w, "w")
-    dev = _device_of(x=xp[0], x_lo=xp[1], w=wp[0], w_lo=wp[1], bias=bias, residual=residual,
-                     out=out, t32=t32, pre=pre)
+    dev = _device_of("x x_lo w w_lo bias residual out t32 pre", *xp, *wp, bias, residual, out, t32,
+                     pre)
     toks, k = xp[0].shape
     rows = wp[0].shape[0]
     if wp[0].shape[1] != k or k == 0 or rows == 0:
@@ -1100,9 +1105,9 @@ def linear(x, w, *, bias=None, act: str = "none", residual=None, out=None, dtype
     if split:
         if out is not None or dtype is not None:
             raise SchemeError("a split output is allocated by the call")
-        out, lo = _pair((toks, feats), dev)
+        out, lo = _pair((toks, feats), xp[0].device)
     elif out is None:
-        out = torch.empty((toks, feats), device=dev,
+        out = torch.empty((toks, feats), device=xp[0].device,
                           dtype=dtype or (torch.bfloat16 if xp[1] is None else torch.float32))
     elif dtype is not None and out.dtype != dtype:
         raise SchemeError(f"out is {out.dtype}, not {dtype}")
@@ -1131,7 +1136,8 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     output of :func:`linear`), the bias gradient float32."""
     code = _act_code(act)
     xp, wp = _parts(x, "x"), _parts(w, "w")
-    dev = _device_of(dy=dy, x=xp[0], x_lo=xp[1], w=wp[0], w_lo=wp[1], pre=pre)
+    dev = _device_of("dy x x_lo w w_lo pre", dy, *xp, *wp, pre)
+    on = dy.device
     toks, k = xp[0].shape
     rows = wp[0].shape[0]
     if wp[0].shape[1] != k or k == 0 or rows == 0 or (act == "swiglu" and rows % 2):
@@ -1148,20 +1154,20 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     if out_dtype not in _LINEAR_OUT:
         raise SchemeError(f"dtype must be float32 or bfloat16, got {out_dtype}")
     x_op, w_op = _operand(xp, "x", False), _operand(wp, "w", False)
-    dx = torch.empty((toks, k), dtype=out_dtype, device=dev)
-    dw = torch.empty((rows, k), dtype=out_dtype, device=dev)
-    db = torch.empty(rows, dtype=torch.float32, device=dev) if bias_grad else None
+    dx = torch.empty((toks, k), dtype=out_dtype, device=on)
+    dw = torch.empty((rows, k), dtype=out_dtype, device=on)
+    db = torch.empty(rows, dtype=torch.float32, device=on) if bias_grad else None
     if toks == 0:
         dw.zero_()
         if db is not None:
             db.zero_()
         return dx, dw, db
     ldz = -(-rows // 8) * 8
-    hi, lo = _pair((toks, ldz), dev)
+    hi, lo = _pair((toks, ldz), on)
     scratch = None
     if bias_grad:
         nbytes = int(lib().mr_act_grad_workspace_bytes(toks, feats, code))
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=on)
     z = None if act == "none" else pre.data_ptr()
     _launch("mr_act_grad", dev, dy.data_ptr(), DTYPES[dy.dtype], ldy, z, ldp, toks, feats, code,
             hi.data_ptr(), lo.data_ptr(), ldz, None if db is None else db.data_ptr(),
