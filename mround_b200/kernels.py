@@ -945,8 +945,8 @@ def _distill(logits, t_logits, t_index, temperature, weight, loss, grad, pair, l
     k = t_logits.shape[1]
     if not 1 <= k <= MAX_TOPK:
         raise SchemeError(f"1 to {MAX_TOPK} teacher logits per row, got {k}")
-    if not 0.0 < float(temperature) < 1e30:
-        raise SchemeError(f"temperature must be positive, got {temperature}")
+    if not 1e-3 <= float(temperature) <= 1e3:
+        raise SchemeError(f"temperature must be 0.001 to 1000, got {temperature}")
     args = (_ptr(t_logits, torch.float32, "t_logits"), _ptr(t_index, torch.int64, "t_index"), k,
             float(temperature), _ptr(weight, torch.float32, "weight", rows))
     if rows:
