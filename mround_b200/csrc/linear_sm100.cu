@@ -45,9 +45,12 @@ constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s per wait
 
 __device__ int g_linear_status = 0;
 
-// Bounded wait; returns false (and raises the status word) on timeout.
+// Bounded wait; returns false (and raises the status word) on timeout.  The
+// clock is read only after many tries: reading it costs as much as a stage.
 __device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+  for (int i = 0; i < 1024; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer();
   for (uint32_t i = 0;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -61,10 +64,64 @@ __device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity) {
   }
 }
 
+// The same by a whole warp, whose lanes go on together.
+__device__ __forceinline__ bool lin_wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, lin_wait(bar, parity));
+}
+
+// Whether the phase is complete, without waiting.
+__device__ __forceinline__ bool lin_peek(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// A ring position: stage and the parity of its current use.
+struct Ring {
+  int s = 0;
+  uint32_t phase;
+  __device__ __forceinline__ explicit Ring(uint32_t p) : phase(p) {}
+  template <int kStages>
+  __device__ __forceinline__ void next() {
+    if (++s == kStages) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 struct LinMaps {
   CUtensorMap a_hi, a_lo, b_hi, b_lo;  // a: features, b: tokens
   int a_kmajor, b_kmajor;
 };
+
+template <int PREC>
+__device__ __forceinline__ void prefetch_maps(const LinMaps& m) {
+  auto fetch = [](const CUtensorMap* p) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(p)) : "memory");
+  };
+  fetch(&m.a_hi);
+  fetch(&m.b_hi);
+  if (PREC == 3) fetch(&m.a_lo);
+  if (PREC >= 2) fetch(&m.b_lo);
+}
 
 // What follows the product.  feats counts outputs (half of the features under
 // SwiGLU, whose up rows start at row `feats`).
@@ -82,6 +139,13 @@ struct LinEpilogue {
 // silu as the block's element-wise kernels compute it
 __device__ __forceinline__ float silu1(float g) { return g / (1.f + expf(-g)); }
 
+// silu to about 2^-20, for a result that is rounded to bf16 at once (2^-8): the
+// exact division made the epilogue of a SwiGLU tile as long as its products at
+// k = 3584 (8 % of the whole).
+__device__ __forceinline__ float silu_rough(float g) {
+  return __fdividef(g, 1.f + __expf(-g));
+}
+
 __device__ __forceinline__ float act1(float z, int act) {
   switch (act) {
     case MR_ACT_SILU: return silu1(z);
@@ -92,32 +156,80 @@ __device__ __forceinline__ float act1(float z, int act) {
   }
 }
 
-// One output: feature f, token t, z without bias (zu: the up row's, SwiGLU).
-template <bool kGated>
-__device__ __forceinline__ void finish(const LinEpilogue& e, int f, int t, float z, float zu) {
-  if (e.bias) {
-    z += e.bias[f];
-    if (kGated) zu += e.bias[e.feats + f];
+// The epilogue of tokens t0 .. t0 + N - 1, as far as `end`, of one feature: v
+// holds z (up: the up row's).
+template <bool kGated, int N>
+__device__ __forceinline__ void finish_run(const LinEpilogue& e, int f, int t0, int end,
+                                           float (&v)[N], const float (&up)[N]) {
+  if (f >= e.feats || t0 >= end) return;
+  const bool rough = e.out_dtype == MR_BF16 && !e.lo && !e.t32;  // bf16 alone is kept
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (!kGated) break;
+    v[i] = (rough ? silu_rough(v[i]) : silu1(v[i])) * up[i];
   }
-  if (e.pre) {
-    e.pre[int64_t(t) * e.ldp + f] = z;
-    if (kGated) e.pre[int64_t(t) * e.ldp + e.feats + f] = zu;
+  if (!kGated && e.act != MR_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = act1(v[i], e.act);
   }
-  float y = kGated ? silu1(z) * zu : act1(z, e.act);
-  if (e.residual) {
-    const int64_t at = int64_t(t) * e.ldr + f;
-    y += e.residual_dtype == MR_F32 ? static_cast<const float*>(e.residual)[at]
-                                    : bf16_to_f32(static_cast<const uint16_t*>(e.residual)[at]);
-  }
-  const int64_t at = int64_t(t) * e.ldo + f;
-  if (e.out_dtype == MR_F32) {
-    static_cast<float*>(e.out)[at] = y;
-  } else {
-    const uint16_t h = f32_to_bf16(y);
-    static_cast<uint16_t*>(e.out)[at] = h;
-    if (e.lo) e.lo[at] = f32_to_bf16(__fsub_rn(y, bf16_to_f32(h)));
-  }
-  if (e.t32) e.t32[at] = tf32_rna(y);
+  auto store = [&](auto whole) {  // whole: all N tokens exist
+    constexpr bool kWhole = decltype(whole)::value;
+    const int n = kWhole ? N : end - t0;
+    if (e.residual) {
+      float r[N];
+      if (e.residual_dtype == MR_F32) {
+        const float* p = static_cast<const float*>(e.residual) + int64_t(t0) * e.ldr + f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = kWhole || i < n ? p[i * e.ldr] : 0.f;
+      } else {
+        const uint16_t* p = static_cast<const uint16_t*>(e.residual) + int64_t(t0) * e.ldr + f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = kWhole || i < n ? bf16_to_f32(p[i * e.ldr]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += r[i];
+    }
+    const int64_t at = int64_t(t0) * e.ldo + f;
+    if (e.out_dtype == MR_F32) {
+      float* p = static_cast<float*>(e.out) + at;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (kWhole || i < n) p[i * e.ldo] = v[i];
+    } else {
+      uint16_t* p = static_cast<uint16_t*>(e.out) + at;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (kWhole || i < n) p[i * e.ldo] = f32_to_bf16(v[i]);
+      if (e.lo) {
+        uint16_t* l = e.lo + at;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (kWhole || i < n)
+            l[i * e.ldo] = f32_to_bf16(__fsub_rn(v[i], bf16_to_f32(f32_to_bf16(v[i]))));
+      }
+    }
+    if (e.t32) {
+      float* p = e.t32 + at;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (kWhole || i < n) p[i * e.ldo] = tf32_rna(v[i]);
+    }
+  };
+  if (t0 + N <= end)
+    store(std::true_type());
+  else
+    store(std::false_type());
+}
+
+// Stores z of tokens t0 .. t0 + N - 1, as far as `end`, for one row of w.
+template <int N>
+__device__ __forceinline__ void store_pre(const LinEpilogue& e, int row, bool on, int t0, int end,
+                                          const float (&v)[N]) {
+  if (!on) return;
+  float* p = e.pre + int64_t(t0) * e.ldp + row;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (t0 + i < end) p[i * e.ldp] = v[i];
 }
 
 // bf16 x bf16 -> float32
@@ -126,13 +238,26 @@ __host__ __device__ constexpr uint32_t lin_idesc(int m, int n, bool a_mn, bool b
          (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
-// 128-byte-swizzled tiles.  K-major: rows of 64 k, 8-row groups 1024 B apart,
-// 16 k are 32 B.  MN-major: boxes of 64 columns x 64 k (8 KB), 8-k groups
-// 1024 B apart, 16 k are 2048 B.
-__device__ __forceinline__ uint64_t lin_desc(uint32_t base, bool kmajor, int ks) {
-  return kmajor ? smem_desc(base + ks * 32, 16, 1024, 2)
-                : smem_desc(base + ks * 2048, 64 * kBK * 2, 1024, 2);
-}
+// Descriptors of 128-byte-swizzled tiles.  K-major: rows of 64 k, 8-row groups
+// 1024 B apart, 16 k are 32 B.  MN-major: boxes of 64 columns x 64 k (8 KB),
+// 8-k groups 1024 B apart, 16 k are 2048 B.  Only the address field (the low
+// word's 14 bits, in 16 bytes) changes from one MMA to the next: the issuing
+// thread adds to it, since building a descriptor per MMA took it as long as
+// the MMAs (450 ns per stage whatever the tile's width).
+struct LinDesc {
+  uint32_t low, high, step;  // step: 16 k further
+  __device__ __forceinline__ LinDesc(uint32_t base, bool kmajor) {
+    const uint64_t d = kmajor ? smem_desc(base, 16, 1024, 2)
+                              : smem_desc(base, 64 * kBK * 2, 1024, 2);
+    low = uint32_t(d);
+    high = uint32_t(d >> 32);
+    step = kmajor ? 32 >> 4 : 2048 >> 4;
+  }
+  // the tile `bytes` further, ks * 16 k in
+  __device__ __forceinline__ uint64_t at(uint32_t bytes16, int ks) const {
+    return (uint64_t(high) << 32) | (low + bytes16 + step * ks);
+  }
+};
 
 template <int BT, int PREC>
 struct SplitCfg {
@@ -204,6 +329,7 @@ __global__ void __launch_bounds__(kSplitThreads)
     }
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_maps<PREC>(maps);
   }
   if (warp == 1) tmem_alloc(tmem_slot, C::kTmemCols);
   tc_fence_before();
@@ -212,11 +338,10 @@ __global__ void __launch_bounds__(kSplitThreads)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0 && lane == 0) {
-    bool ok = true;
-    for (int kt = kt0; kt < kt1; ++kt) {
-      const int it = kt - kt0, s = it % C::kStages;
-      if (it >= C::kStages) ok = lin_wait(&empty[s], (it / C::kStages - 1) & 1);
-      if (!ok) break;
+    Ring ring(1);  // of the stages' previous use; the first passes at once
+    for (int kt = kt0; kt < kt1; ++kt, ring.next<C::kStages>()) {
+      const int s = ring.s;
+      if (!lin_wait(&empty[s], ring.phase)) break;
       uint8_t* st = smem + s * C::kStage;
       mbar_expect_tx(&full[s], C::kStage);
       load_features<kGated>(st, &maps.a_hi, &full[s], maps.a_kmajor, f0, e.feats, kt * kBK);
@@ -228,29 +353,34 @@ __global__ void __launch_bounds__(kSplitThreads)
       if constexpr (C::kBParts == 2)
         load_rows<BT>(sb + C::kBBytes, &maps.b_lo, &full[s], maps.b_kmajor, t0, kt * kBK);
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     const uint32_t idesc = lin_idesc(128, BT, !maps.a_kmajor, !maps.b_kmajor);
-    bool ok = true;
+    const LinDesc da(smem_u32(smem), maps.a_kmajor);
+    const LinDesc db(smem_u32(smem) + kABytes * C::kAParts, maps.b_kmajor);
+    const bool leader = elect_one();
+    Ring ring(0);
+    bool ready = false;
     for (int kt = kt0; kt < kt1; ++kt) {
-      const int it = kt - kt0, s = it % C::kStages;
-      ok = lin_wait(&full[s], (it / C::kStages) & 1);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t a_hi = smem_u32(smem + s * C::kStage);
-      const uint32_t b_hi = a_hi + kABytes * C::kAParts;
+      if (!ready && !lin_wait_warp(&full[ring.s], ring.phase)) break;
+      const int s = ring.s;
+      ring.next<C::kStages>();
+      // looked at before this stage's MMAs go out, read after them
+      const bool peeked = kt + 1 < kt1 && lin_peek(&full[ring.s], ring.phase);
+      const uint32_t off = uint32_t(s) * (C::kStage >> 4);
+      if (leader) {
 #pragma unroll
-      for (int ks = 0; ks < kBK / 16; ++ks) {
-        const uint64_t dah = lin_desc(a_hi, maps.a_kmajor, ks);
-        const uint64_t dbh = lin_desc(b_hi, maps.b_kmajor, ks);
-        umma_bf16(tmem, dah, dbh, idesc, (it > 0 || ks > 0) ? 1u : 0u);
-        if constexpr (PREC == 3)
-          umma_bf16(tmem, lin_desc(a_hi + kABytes, maps.a_kmajor, ks), dbh, idesc, 1u);
-        if constexpr (PREC >= 2)
-          umma_bf16(tmem, dah, lin_desc(b_hi + C::kBBytes, maps.b_kmajor, ks), idesc, 1u);
+        for (int ks = 0; ks < kBK / 16; ++ks) {
+          const uint64_t dah = da.at(off, ks), dbh = db.at(off, ks);
+          umma_bf16(tmem, dah, dbh, idesc, (kt > kt0 || ks > 0) ? 1u : 0u);
+          if constexpr (PREC == 3) umma_bf16(tmem, da.at(off + (kABytes >> 4), ks), dbh, idesc, 1u);
+          if constexpr (PREC >= 2)
+            umma_bf16(tmem, dah, db.at(off + (C::kBBytes >> 4), ks), idesc, 1u);
+        }
+        umma_commit(&empty[s]);
       }
-      umma_commit(&empty[s]);
+      ready = __all_sync(0xffffffffu, peeked);
     }
-    umma_commit(done);
+    if (leader) umma_commit(done);
   }
   __syncwarp();
   // every MMA of this CTA has completed: the accumulator may be read, and the
@@ -277,25 +407,44 @@ __global__ void __launch_bounds__(kSplitThreads)
   __syncwarp();
   if (splits > 1) cluster_sync_all(); else __syncthreads();
   if (ok) {
-    const int share = (toks + splits - 1) / splits;
+    // each thread a feature and runs of kRun tokens, loaded together
+    constexpr int kRun = BT >= 64 ? 8 : 4;
+    const int share = ((toks + splits - 1) / splits + kRun - 1) / kRun * kRun;
     const int first = rank * share, last = min(first + share, toks);
     const int f = threadIdx.x % kOut;
-    const uint32_t base = smem_u32(partial);
-    if (f0 + f < e.feats) {
-      for (int t = first + int(threadIdx.x) / kOut; t < last; t += kSplitThreads / kOut) {
-        float z = 0.f, zu = 0.f;
-        if (splits == 1) {
-          z = partial[t * kTileF + f];
-          if (kGated) zu = partial[t * kTileF + kOut + f];
-        } else {
-          for (int s = 0; s < splits; ++s) {
-            const uint32_t at = map_rank(base + uint32_t(t * kTileF + f) * 4u, s);
-            z += ld_cluster(at);
-            if (kGated) zu += ld_cluster(at + kOut * 4u);
+    const uint32_t base = smem_u32(partial) + uint32_t(f) * 4u;
+    const bool on = f0 + f < e.feats;
+    float bias = 0.f, bias_up = 0.f;
+    if (e.bias && on) {
+      bias = e.bias[f0 + f];
+      if (kGated) bias_up = e.bias[e.feats + f0 + f];
+    }
+    for (int t = first + int(threadIdx.x) / kOut * kRun; t < last;
+         t += kSplitThreads / kOut * kRun) {
+      float z[kRun] = {}, zu[kRun] = {};
+      for (int s = 0; s < splits; ++s) {
+        // plain loads of this CTA's own memory where nothing is divided
+        const uint32_t from = (splits > 1 ? map_rank(base, s) : base) + uint32_t(t * kTileF) * 4u;
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+          if (t + i < last) {
+            z[i] += ld_cluster(from + uint32_t(i * kTileF) * 4u);
+            if (kGated) zu[i] += ld_cluster(from + uint32_t(i * kTileF + kOut) * 4u);
           }
         }
-        finish<kGated>(e, f0 + f, t0 + t, z, zu);
       }
+      if (e.bias) {
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+          z[i] += bias;
+          if (kGated) zu[i] += bias_up;
+        }
+      }
+      if (e.pre) {
+        store_pre(e, f0 + f, on, t0 + t, t0 + last, z);
+        if (kGated) store_pre(e, e.feats + f0 + f, on, t0 + t, t0 + last, zu);
+      }
+      finish_run<kGated, kRun>(e, f0 + f, t0 + t, t0 + last, z, zu);
     }
   }
   if (!ok) {  // let issued copies land before the CTA exits
@@ -315,19 +464,20 @@ __global__ void __launch_bounds__(kSplitThreads)
 
 // ---------------------------------------------------------------- wide kernel
 // Many tokens: a persistent kernel of CTA pairs.  A pair computes 256 features
-// x 256 tokens with tcgen05.mma.cta_group::2 (M = 256, N = 256): each CTA
-// stages its 128 feature rows and half of the token rows and keeps its 128
-// lanes x 256 columns of the accumulator, so a stage holds 256 rows of k for
-// 2 x 128 x 256 flops per k and CTA -- a third less than a 128 x 256 tile of
-// one CTA.  Two accumulators: the epilogue of one tile overlaps the MMAs of
-// the next.
+// x BT tokens (256, or fewer where that shortens the schedule) with
+// tcgen05.mma.cta_group::2 (M = 256, N = BT): each CTA stages its 128 feature
+// rows and half of the token rows and keeps its 128 lanes x BT columns of the
+// accumulator, so a stage holds 256 rows of k for 2 x 128 x 256 flops per k and
+// CTA -- a third less than a 128 x 256 tile of one CTA.  Two accumulators: the
+// epilogue of one tile, by eight warps (SiLU's exponential and division took
+// four warps as long as the MMAs of k = 3584), overlaps the MMAs of the next.
 //
 // The leader (rank 0) issues the MMAs for both.  Both CTAs' loads complete on
 // the leader's "full" barrier; the MMAs' commits free the stage, and publish
 // the accumulator, on the barriers of both; the epilogue warps of both arrive
 // on the leader's "tmem_empty".
-constexpr int kWideThreads = 192;
-constexpr int kWideT = 256;          // tokens per tile
+constexpr int kWideThreads = 320;
+constexpr int kWideT = 256;          // most tokens per tile
 constexpr int kWideBufs = 2;         // accumulators of 256 columns
 
 template <int PREC>
@@ -337,8 +487,8 @@ struct WideCfg {
   static constexpr int kBBytes = kWideT / 2 * kBK * 2;
   static constexpr int kStage = kABytes * kAParts + kBBytes * kBParts;
   static constexpr int kStages = 192 * 1024 / kStage;
-  // SwiGLU: two buffers of 32 x 32 float32 in each direction per pair of warps
-  static constexpr int kExchange = 2 * 2 * 2 * 32 * 32 * 4;
+  // SwiGLU: two buffers of 16 x 32 float32 in each direction per pair of warps
+  static constexpr int kExchange = 4 * 2 * 2 * 16 * 32 * 4;
   static constexpr int kSmem = kStages * kStage + kExchange + 1024 /* align */ + 256;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
 };
@@ -352,15 +502,14 @@ __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map,
       : "memory");
 }
 
-// One operand part of ROWS rows (features or tokens) of a stage.
-template <int ROWS>
+// One operand part of a stage: rows as high as the map's box (K-major), or
+// `chunks` of 64 rows (MN-major).
 __device__ __forceinline__ void load_pair_rows(uint8_t* dst, const CUtensorMap* map, uint32_t bar,
-                                               bool kmajor, int row0, int k0) {
+                                               bool kmajor, int row0, int k0, int chunks) {
   if (kmajor) {
     tma_load_pair(dst, map, bar, k0, row0);
   } else {
-#pragma unroll
-    for (int c = 0; c < ROWS / 64; ++c)
+    for (int c = 0; c < chunks; ++c)
       tma_load_pair(dst + c * 64 * kBK * 2, map, bar, row0 + c * 64, k0);
   }
 }
@@ -373,7 +522,7 @@ __device__ __forceinline__ void load_pair_features(uint8_t* dst, const CUtensorM
     tma_load_pair(dst, map, bar, k0, f0);
     tma_load_pair(dst + kABytes / 2, map, bar, k0, up0 + f0);
   } else {
-    load_pair_rows<kTileF>(dst, map, bar, kmajor, f0, k0);
+    load_pair_rows(dst, map, bar, kmajor, f0, k0, kTileF / 64);
   }
 }
 
@@ -399,13 +548,13 @@ __device__ __forceinline__ void arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Whether `ok` holds in all four epilogue warps.
+// Whether `ok` holds in all eight epilogue warps.
 __device__ __forceinline__ bool epilogue_agrees(bool ok) {
   int all;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.s32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred.aligned q, 3, 128, p;\n\t"
+      "barrier.cta.red.and.pred.aligned q, 5, 256, p;\n\t"
       "selp.s32 %0, 1, 0, q;\n\t}"
       : "=r"(all)
       : "r"(int(ok))
@@ -425,73 +574,10 @@ __device__ __forceinline__ void wide_tile(int t, int f_tiles, int t_tiles, int* 
   *ft = r / rows;
 }
 
-// The epilogue of 32 tokens of one feature (lane): v holds z without bias.
-template <bool kGated>
-__device__ __forceinline__ void finish32(const LinEpilogue& e, int f, int t0, float (&v)[32],
-                                         const float (&up)[32]) {
-  const int n = min(32, e.toks - t0);
-  if (f >= e.feats) return;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = kGated ? silu1(v[i]) * up[i] : v[i];
-  if (!kGated && e.act != MR_ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act1(v[i], e.act);
-  }
-  if (e.residual) {
-    float r[32];
-    if (e.residual_dtype == MR_F32) {
-      const float* p = static_cast<const float*>(e.residual) + int64_t(t0) * e.ldr + f;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) r[i] = i < n ? p[i * e.ldr] : 0.f;
-    } else {
-      const uint16_t* p = static_cast<const uint16_t*>(e.residual) + int64_t(t0) * e.ldr + f;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) r[i] = i < n ? bf16_to_f32(p[i * e.ldr]) : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] += r[i];
-  }
-  const int64_t at = int64_t(t0) * e.ldo + f;
-  if (e.out_dtype == MR_F32) {
-    float* p = static_cast<float*>(e.out) + at;
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) p[i * e.ldo] = v[i];
-  } else {
-    uint16_t* p = static_cast<uint16_t*>(e.out) + at;
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) p[i * e.ldo] = f32_to_bf16(v[i]);
-    if (e.lo) {
-      uint16_t* l = e.lo + at;
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < n) l[i * e.ldo] = f32_to_bf16(__fsub_rn(v[i], bf16_to_f32(f32_to_bf16(v[i]))));
-    }
-  }
-  if (e.t32) {
-    float* p = e.t32 + at;
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) p[i * e.ldo] = tf32_rna(v[i]);
-  }
-}
-
-// Stores 32 tokens of z for one feature (row of w).
-__device__ __forceinline__ void store_pre(const LinEpilogue& e, int row, bool on, int t0,
-                                          const float (&v)[32]) {
-  const int n = min(32, e.toks - t0);
-  if (!on) return;
-  float* p = e.pre + int64_t(t0) * e.ldp + row;
-#pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (i < n) p[i * e.ldp] = v[i];
-}
-
 template <int PREC, bool kGated>
 __global__ void __launch_bounds__(kWideThreads, 1) __cluster_dims__(2, 1, 1)
     linear_wide_kernel(const __grid_constant__ LinMaps maps,
-                       const __grid_constant__ LinEpilogue e, int k, int f_tiles, int t_tiles) {
+                       const __grid_constant__ LinEpilogue e, int k, int bt, int f_tiles, int t_tiles) {
   using C = WideCfg<PREC>;
   constexpr int kOut = kGated ? kTileF / 2 : kTileF;  // outputs per CTA
   extern __shared__ uint8_t smem_raw[];
@@ -516,9 +602,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) __cluster_dims__(2, 1, 1)
     }
     for (int b = 0; b < kWideBufs; ++b) {
       mbar_init(&tmem_full[b], 1);
-      mbar_init(&tmem_empty[b], 8);  // four epilogue warps of each CTA
+      mbar_init(&tmem_empty[b], 16);  // eight epilogue warps of each CTA
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_maps<PREC>(maps);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -536,70 +623,84 @@ __global__ void __launch_bounds__(kWideThreads, 1) __cluster_dims__(2, 1, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
+      // of both CTAs; fewer than 256 tokens fill part of a stage
+      const uint32_t stage_bytes =
+          2 * (kABytes * C::kAParts + uint32_t(bt / 2) * kBK * 2 * C::kBParts);
+      const uint32_t leader_full = map_rank(smem_u32(full), 0);
+      Ring ring(1);  // of the stages' previous use; the first passes at once
       for (int t = first; t < total && ok; t += pairs) {
         int ft, tt;
         wide_tile(t, f_tiles, t_tiles, &ft, &tt);
-        const int f0 = (ft * 2 + rank) * kOut, t0 = tt * kWideT + rank * (kWideT / 2);
-        for (int kt = 0; kt < k_tiles; ++kt, ++it) {
-          const int s = it % C::kStages;
-          if (it >= C::kStages) ok = lin_wait(&empty[s], (it / C::kStages - 1) & 1);
+        const int f0 = (ft * 2 + rank) * kOut, t0 = tt * bt + rank * (bt / 2);
+        for (int kt = 0; kt < k_tiles; ++kt, ring.next<C::kStages>()) {
+          const int s = ring.s;
+          ok = lin_wait(&empty[s], ring.phase);
           if (!ok) break;
           uint8_t* st = smem + s * C::kStage;
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * C::kStage);
-          const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_expect_tx(&full[s], stage_bytes);
+          const uint32_t bar = leader_full + uint32_t(s) * 8u;
           load_pair_features<kGated>(st, &maps.a_hi, bar, maps.a_kmajor, f0, e.feats, kt * kBK);
           if constexpr (C::kAParts == 2)
             load_pair_features<kGated>(st + kABytes, &maps.a_lo, bar, maps.a_kmajor, f0, e.feats,
                                        kt * kBK);
           uint8_t* sb = st + kABytes * C::kAParts;
-          load_pair_rows<kWideT / 2>(sb, &maps.b_hi, bar, maps.b_kmajor, t0, kt * kBK);
+          load_pair_rows(sb, &maps.b_hi, bar, maps.b_kmajor, t0, kt * kBK, bt / 128);
           if constexpr (C::kBParts == 2)
-            load_pair_rows<kWideT / 2>(sb + C::kBBytes, &maps.b_lo, bar, maps.b_kmajor, t0,
-                                       kt * kBK);
+            load_pair_rows(sb + C::kBBytes, &maps.b_lo, bar, maps.b_kmajor, t0, kt * kBK, bt / 128);
         }
       }
-      // the last use of every stage has been signalled before this CTA leaves
-      for (int i = max(0, it - C::kStages); i < it && ok; ++i)
-        ok = lin_wait(&empty[i % C::kStages], (i / C::kStages) & 1);
+      // every stage's last use has been signalled before this CTA leaves
+      for (int i = 0; i < C::kStages && ok; ++i, ring.next<C::kStages>())
+        ok = lin_wait(&empty[ring.s], ring.phase);
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = lin_idesc(256, kWideT, !maps.a_kmajor, !maps.b_kmajor);
-      int it = 0, j = 0;
+    if (rank == 0) {
+      const uint32_t idesc = lin_idesc(256, bt, !maps.a_kmajor, !maps.b_kmajor);
+      const LinDesc da(smem_u32(smem), maps.a_kmajor);
+      const LinDesc db(smem_u32(smem) + kABytes * C::kAParts, maps.b_kmajor);
+      const bool leader = elect_one();
+      Ring ring(0);
+      bool ready = false;
+      int j = 0;
       for (int t = first; t < total && ok; t += pairs, ++j) {
         const int b = j % kWideBufs;
-        if (j >= kWideBufs) ok = lin_wait(&tmem_empty[b], (j / kWideBufs - 1) & 1);
+        if (j >= kWideBufs) ok = lin_wait_warp(&tmem_empty[b], (j / kWideBufs - 1) & 1);
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + uint32_t(b * kWideT);
-        for (int kt = 0; kt < k_tiles; ++kt, ++it) {
-          const int s = it % C::kStages;
-          ok = lin_wait(&full[s], (it / C::kStages) & 1);
+        for (int kt = 0; kt < k_tiles; ++kt) {
+          if (!ready) ok = lin_wait_warp(&full[ring.s], ring.phase);
           if (!ok) break;
-          tc_fence_after();
-          const uint32_t a_hi = smem_u32(smem + s * C::kStage);
-          const uint32_t b_hi = a_hi + kABytes * C::kAParts;
+          const int s = ring.s;
+          ring.next<C::kStages>();
+          // looked at before this stage's MMAs go out, read after them
+          const bool peeked = lin_peek(&full[ring.s], ring.phase);
+          const uint32_t off = uint32_t(s) * (C::kStage >> 4);
+          if (leader) {
 #pragma unroll
-          for (int ks = 0; ks < kBK / 16; ++ks) {
-            const uint64_t dah = lin_desc(a_hi, maps.a_kmajor, ks);
-            const uint64_t dbh = lin_desc(b_hi, maps.b_kmajor, ks);
-            umma_pair(d, dah, dbh, idesc, (kt > 0 || ks > 0) ? 1u : 0u);
-            if constexpr (PREC == 3)
-              umma_pair(d, lin_desc(a_hi + kABytes, maps.a_kmajor, ks), dbh, idesc, 1u);
-            if constexpr (PREC >= 2)
-              umma_pair(d, dah, lin_desc(b_hi + C::kBBytes, maps.b_kmajor, ks), idesc, 1u);
+            for (int ks = 0; ks < kBK / 16; ++ks) {
+              const uint64_t dah = da.at(off, ks), dbh = db.at(off, ks);
+              umma_pair(d, dah, dbh, idesc, (kt > 0 || ks > 0) ? 1u : 0u);
+              if constexpr (PREC == 3)
+                umma_pair(d, da.at(off + (kABytes >> 4), ks), dbh, idesc, 1u);
+              if constexpr (PREC >= 2)
+                umma_pair(d, dah, db.at(off + (C::kBBytes >> 4), ks), idesc, 1u);
+            }
+            commit_pair(&empty[s]);
           }
-          commit_pair(&empty[s]);
+          ready = __all_sync(0xffffffffu, peeked);
         }
         if (!ok) break;
-        commit_pair(&tmem_full[b]);
+        if (leader) commit_pair(&tmem_full[b]);
+        __syncwarp();
       }
     }
   } else {
     const int quarter = warp & 3;  // lanes 32 quarter .. + 31
+    const int odd = warp >= 6;     // warps 2-5 take the even 32-token runs, 6-9 the odd ones
     const int l = quarter * 32 + lane;
-    const int half = quarter >> 1, pair = quarter & 1;  // SwiGLU: gate (0) or up (1) rows
+    const int half = quarter >> 1;  // SwiGLU: gate (0) or up (1) rows
+    const int pair = (quarter & 1) + 2 * odd;  // of warps with the same features and tokens
     const uint32_t empty_at = map_rank(smem_u32(tmem_empty), 0);
     int j = 0;
     for (int t = first; t < total; t += pairs, ++j) {
@@ -610,62 +711,47 @@ __global__ void __launch_bounds__(kWideThreads, 1) __cluster_dims__(2, 1, 1)
            *reinterpret_cast<volatile int*>(&g_linear_status) == 0;
       tc_fence_after();
       __syncwarp();
-      // the four warps go on, or give up, together: they wait for one another below
+      // the eight warps go on, or give up, together: they wait for one another below
       ok = epilogue_agrees(ok);
       if (!ok) break;
-      const int f0 = (ft * 2 + rank) * kOut, t0 = tt * kWideT;
+      const int f0 = (ft * 2 + rank) * kOut, t0 = tt * bt;
       const uint32_t lanes = tmem + uint32_t(b * kWideT) + (uint32_t(quarter * 32) << 16);
       const int f = f0 + (kGated ? l % kOut : l);
       const int row = kGated ? f + half * e.feats : f;  // row of w
       const bool on = f < e.feats;
       const float bias = e.bias && on ? e.bias[row] : 0.f;
-      if constexpr (!kGated) {
+      int turn = 0;
 #pragma unroll 1
-        for (int col = 0; col < kWideT && t0 + col < e.toks; col += 32) {
-          float v[32];
-          __syncwarp();
-          tmem_ld32(lanes + col, v);
-          if (e.bias) {
+      for (int col = odd * 32; col < bt && t0 + col < e.toks; col += 64, turn ^= 1) {
+        float v[32];
+        __syncwarp();
+        tmem_ld32(lanes + col, v);
+        if (e.bias) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += bias;
-          }
-          if (e.pre) store_pre(e, row, on, t0 + col, v);
-          finish32<false>(e, f, t0 + col, v, v);
+          for (int i = 0; i < 32; ++i) v[i] += bias;
         }
-      } else {
-        // warps q (gate) and q + 2 (up) hold the same features: of every 64
-        // tokens the gate warp finishes the first 32, the up warp the others
-#pragma unroll 1
-        for (int col = 0; col < kWideT; col += 64) {
-          float mine[32], give[32];
-          __syncwarp();
-          tmem_ld32(lanes + col + half * 32, mine);
-          tmem_ld32(lanes + col + (1 - half) * 32, give);
-          if (e.bias) {
+        if (e.pre) store_pre(e, row, on, t0 + col, e.toks, v);
+        if constexpr (!kGated) {
+          finish_run<false, 32>(e, f, t0 + col, e.toks, v, v);
+        } else {
+          // warps q (gate) and q + 2 (up) hold the same features: the gate warp
+          // finishes the first 16 tokens of the run, the up warp the others
+          float* box = exchange + (pair * 2 + turn) * 1024;
+          float* to = box + (1 - half) * 512;
+          float* from = box + half * 512;
+          float mine[16], other[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              mine[i] += bias;
-              give[i] += bias;
-            }
+          for (int i = 0; i < 16; ++i) {
+            mine[i] = half ? v[16 + i] : v[i];
+            to[i * 32 + lane] = half ? v[i] : v[16 + i];
           }
-          const int mine0 = t0 + col + half * 32, give0 = t0 + col + (1 - half) * 32;
-          if (e.pre) {
-            store_pre(e, row, on, mine0, mine);
-            store_pre(e, row, on, give0, give);
-          }
-          float* box = exchange + ((col >> 6) & 1) * 4096 + pair * 2048;
-          float* to = box + (1 - half) * 1024;
-          float* from = box + half * 1024;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) to[i * 32 + lane] = give[i];
           asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
-          float other[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) other[i] = from[i * 32 + lane];
+          for (int i = 0; i < 16; ++i) other[i] = from[i * 32 + lane];
           if (half == 0)
-            finish32<true>(e, f, mine0, mine, other);
+            finish_run<true, 16>(e, f, t0 + col, e.toks, mine, other);
           else
-            finish32<true>(e, f, mine0, other, mine);
+            finish_run<true, 16>(e, f, t0 + col + 16, e.toks, other, mine);
         }
       }
       tc_fence_before();
@@ -738,8 +824,8 @@ int launch_split(const LinMaps& maps, const LinEpilogue& e, int k, int splits, i
 }
 
 template <int PREC, bool kGated>
-int launch_wide(const LinMaps& maps, const LinEpilogue& e, int k, int64_t f_tiles, int64_t t_tiles,
-                cudaStream_t stream) {
+int launch_wide(const LinMaps& maps, const LinEpilogue& e, int k, int bt, int64_t f_tiles,
+                int64_t t_tiles, cudaStream_t stream) {
   using C = WideCfg<PREC>;
   static std::atomic<bool> configured[kMaxDevices];
   auto kernel = linear_wide_kernel<PREC, kGated>;
@@ -748,19 +834,22 @@ int launch_wide(const LinMaps& maps, const LinEpilogue& e, int k, int64_t f_tile
   if (f_tiles * t_tiles > 0x7fffffff) return MR_ERR_ARGUMENT;
   const int64_t pairs = sm_count() / 2;
   const int64_t grid = 2 * (f_tiles * t_tiles < pairs ? f_tiles * t_tiles : pairs);
-  kernel<<<unsigned(grid), kWideThreads, C::kSmem, stream>>>(maps, e, k, int(f_tiles), int(t_tiles));
+  kernel<<<unsigned(grid), kWideThreads, C::kSmem, stream>>>(maps, e, k, bt, int(f_tiles),
+                                                            int(t_tiles));
   return launch_status();
 }
 
 struct LinPlan {
-  int bt, splits;  // bt = kWideT: the wide kernel
+  int bt, splits;
+  bool wide;
 };
 
 // Token tile: the smallest that holds the tokens, up to 128.  K is divided so
 // that about two CTAs per SM are at work, each with at least four K slices.
 LinPlan plan_linear(int64_t f_tiles, int64_t toks, int64_t k, int b_kmajor, int splits) {
   LinPlan p;
-  if (splits <= 1 && toks >= 512) return {kWideT, 1};
+  if (splits <= 1 && toks >= 512) return {kWideT, 1, true};
+  p.wide = false;
   p.bt = toks <= 16 ? 16 : toks <= 32 ? 32 : toks <= 64 ? 64 : 128;
   if (!b_kmajor && p.bt < 64) p.bt = 64;  // MN-major boxes are 64 tokens wide
   const int64_t tiles = f_tiles * ((toks + p.bt - 1) / p.bt);
@@ -782,17 +871,17 @@ int run_linear(LinMaps& maps, const LinEpilogue& e, const void* a_hi, const void
   constexpr int kOut = kGated ? kTileF / 2 : kTileF;
   const int64_t f_tiles = (int64_t(e.feats) + kOut - 1) / kOut;
   const LinPlan p = plan_linear(f_tiles, e.toks, k, maps.b_kmajor, splits);
-  const bool wide = p.bt == kWideT;
-  const int t_box = wide ? kWideT / 2 : p.bt;
+  const int t_box = p.wide ? p.bt / 2 : p.bt;
   const bool good =
       lin_map(&maps.a_hi, a_hi, maps.a_kmajor, rows_a, k, lda, kOut) &&
       lin_map(&maps.b_hi, b_hi, maps.b_kmajor, e.toks, k, ldb, t_box) &&
       (PREC < 3 || lin_map(&maps.a_lo, a_lo, maps.a_kmajor, rows_a, k, lda, kOut)) &&
       (PREC < 2 || lin_map(&maps.b_lo, b_lo, maps.b_kmajor, e.toks, k, ldb, t_box));
   if (!good) return MR_ERR_ALIGNMENT;
-  if (wide)
-    return launch_wide<PREC, kGated>(maps, e, int(k), (int64_t(e.feats) + 2 * kOut - 1) / (2 * kOut),
-                                     (int64_t(e.toks) + kWideT - 1) / kWideT, stream);
+  if (p.wide)
+    return launch_wide<PREC, kGated>(maps, e, int(k), p.bt,
+                                     (int64_t(e.feats) + 2 * kOut - 1) / (2 * kOut),
+                                     (int64_t(e.toks) + p.bt - 1) / p.bt, stream);
   const int64_t t_tiles = (int64_t(e.toks) + p.bt - 1) / p.bt;
   switch (p.bt) {
     case 16: return launch_split<16, PREC, kGated>(maps, e, int(k), p.splits, f_tiles, t_tiles, stream);
