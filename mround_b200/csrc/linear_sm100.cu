@@ -24,12 +24,18 @@
 // reading the partials over distributed shared memory in rank order, so the
 // result does not depend on timing and needs no workspace.
 //
-// Roles (256 threads): warp 0 one lane TMA producer; warp 1 TMEM and one lane
-// MMA issuer; warps 2-5 read the accumulator; all warps finish the outputs.
+// Roles (256 threads): warps 0 and 6 TMA producers (features, tokens); warp 1
+// TMEM and MMA issuer; warps 2-5 read the accumulator; all finish the outputs.
+// Producers and issuer run as whole warps with one elected lane, so that their
+// operands stay in uniform registers, and look at the next stage's barrier
+// before they issue this one's work.
 // Every mbarrier wait is bounded: one that gives up sets the status word that
 // mr_gemm_status reads, and every role goes on to the barriers at the end.
 
 #include <string.h>
+
+#include <algorithm>
+#include <cmath>
 
 #include "linear.h"
 #include "rowtypes.cuh"
@@ -324,7 +330,7 @@ __global__ void __launch_bounds__(kSplitThreads)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 2);  // two producers
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
@@ -337,21 +343,32 @@ __global__ void __launch_bounds__(kSplitThreads)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0 || warp == 6) {
+    // features by warp 0, tokens by warp 6: one warp issuing both, a lane of its
+    // own, took 300 ns per stage, this takes 175
+    const bool leader = elect_one();
     Ring ring(1);  // of the stages' previous use; the first passes at once
-    for (int kt = kt0; kt < kt1; ++kt, ring.next<C::kStages>()) {
+    bool ready = false;
+    for (int kt = kt0; kt < kt1; ++kt) {
       const int s = ring.s;
-      if (!lin_wait(&empty[s], ring.phase)) break;
-      uint8_t* st = smem + s * C::kStage;
-      mbar_expect_tx(&full[s], C::kStage);
-      load_features<kGated>(st, &maps.a_hi, &full[s], maps.a_kmajor, f0, e.feats, kt * kBK);
-      if constexpr (C::kAParts == 2)
-        load_features<kGated>(st + kABytes, &maps.a_lo, &full[s], maps.a_kmajor, f0, e.feats,
-                              kt * kBK);
-      uint8_t* sb = st + kABytes * C::kAParts;
-      load_rows<BT>(sb, &maps.b_hi, &full[s], maps.b_kmajor, t0, kt * kBK);
-      if constexpr (C::kBParts == 2)
-        load_rows<BT>(sb + C::kBBytes, &maps.b_lo, &full[s], maps.b_kmajor, t0, kt * kBK);
+      if (!ready && !lin_wait_warp(&empty[s], ring.phase)) break;
+      ring.next<C::kStages>();
+      const bool peeked = lin_peek(&empty[ring.s], ring.phase);
+      if (leader && warp == 0) {
+        uint8_t* st = smem + s * C::kStage;
+        mbar_expect_tx(&full[s], kABytes * C::kAParts);
+        load_features<kGated>(st, &maps.a_hi, &full[s], maps.a_kmajor, f0, e.feats, kt * kBK);
+        if constexpr (C::kAParts == 2)
+          load_features<kGated>(st + kABytes, &maps.a_lo, &full[s], maps.a_kmajor, f0, e.feats,
+                                kt * kBK);
+      } else if (leader) {
+        mbar_expect_tx(&full[s], C::kBBytes * C::kBParts);
+        uint8_t* sb = smem + s * C::kStage + kABytes * C::kAParts;
+        load_rows<BT>(sb, &maps.b_hi, &full[s], maps.b_kmajor, t0, kt * kBK);
+        if constexpr (C::kBParts == 2)
+          load_rows<BT>(sb + C::kBBytes, &maps.b_lo, &full[s], maps.b_kmajor, t0, kt * kBK);
+      }
+      ready = __all_sync(0xffffffffu, peeked);
     }
   } else if (warp == 1) {
     const uint32_t idesc = lin_idesc(128, BT, !maps.a_kmajor, !maps.b_kmajor);
@@ -622,20 +639,24 @@ __global__ void __launch_bounds__(kWideThreads, 1) __cluster_dims__(2, 1, 1)
   bool ok = true;
 
   if (warp == 0) {
-    if (lane == 0) {
-      // of both CTAs; fewer than 256 tokens fill part of a stage
-      const uint32_t stage_bytes =
-          2 * (kABytes * C::kAParts + uint32_t(bt / 2) * kBK * 2 * C::kBParts);
-      const uint32_t leader_full = map_rank(smem_u32(full), 0);
-      Ring ring(1);  // of the stages' previous use; the first passes at once
-      for (int t = first; t < total && ok; t += pairs) {
-        int ft, tt;
-        wide_tile(t, f_tiles, t_tiles, &ft, &tt);
-        const int f0 = (ft * 2 + rank) * kOut, t0 = tt * bt + rank * (bt / 2);
-        for (int kt = 0; kt < k_tiles; ++kt, ring.next<C::kStages>()) {
-          const int s = ring.s;
-          ok = lin_wait(&empty[s], ring.phase);
-          if (!ok) break;
+    // of both CTAs; fewer than 256 tokens fill part of a stage
+    const uint32_t stage_bytes =
+        2 * (kABytes * C::kAParts + uint32_t(bt / 2) * kBK * 2 * C::kBParts);
+    const uint32_t leader_full = map_rank(smem_u32(full), 0);
+    const bool leader = elect_one();
+    Ring ring(1);  // of the stages' previous use; the first passes at once
+    bool ready = false;
+    for (int t = first; t < total && ok; t += pairs) {
+      int ft, tt;
+      wide_tile(t, f_tiles, t_tiles, &ft, &tt);
+      const int f0 = (ft * 2 + rank) * kOut, t0 = tt * bt + rank * (bt / 2);
+      for (int kt = 0; kt < k_tiles; ++kt) {
+        const int s = ring.s;
+        if (!ready) ok = lin_wait_warp(&empty[s], ring.phase);
+        if (!ok) break;
+        ring.next<C::kStages>();
+        const bool peeked = lin_peek(&empty[ring.s], ring.phase);
+        if (leader) {
           uint8_t* st = smem + s * C::kStage;
           if (rank == 0) mbar_expect_tx(&full[s], stage_bytes);
           const uint32_t bar = leader_full + uint32_t(s) * 8u;
@@ -648,11 +669,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) __cluster_dims__(2, 1, 1)
           if constexpr (C::kBParts == 2)
             load_pair_rows(sb + C::kBBytes, &maps.b_lo, bar, maps.b_kmajor, t0, kt * kBK, bt / 128);
         }
+        ready = __all_sync(0xffffffffu, peeked);
       }
-      // every stage's last use has been signalled before this CTA leaves
-      for (int i = 0; i < C::kStages && ok; ++i, ring.next<C::kStages>())
-        ok = lin_wait(&empty[ring.s], ring.phase);
     }
+    // every stage's last use has been signalled before this CTA leaves
+    for (int i = 0; i < C::kStages && ok; ++i, ring.next<C::kStages>())
+      ok = lin_wait_warp(&empty[ring.s], ring.phase);
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t idesc = lin_idesc(256, bt, !maps.a_kmajor, !maps.b_kmajor);
@@ -844,24 +866,69 @@ struct LinPlan {
   bool wide;
 };
 
-// Token tile: the smallest that holds the tokens, up to 128.  K is divided so
-// that about two CTAs per SM are at work, each with at least four K slices.
-LinPlan plan_linear(int64_t f_tiles, int64_t toks, int64_t k, int b_kmajor, int splits) {
-  LinPlan p;
-  if (splits <= 1 && toks >= 512) return {kWideT, 1, true};
-  p.wide = false;
-  p.bt = toks <= 16 ? 16 : toks <= 32 ? 32 : toks <= 64 ? 64 : 128;
-  if (!b_kmajor && p.bt < 64) p.bt = 64;  // MN-major boxes are 64 tokens wide
-  const int64_t tiles = f_tiles * ((toks + p.bt - 1) / p.bt);
-  const int64_t k_tiles = (k + kBK - 1) / kBK;
-  p.splits = splits;
-  if (!splits) {
-    const int64_t at_once = int64_t(sm_count()) * (p.bt <= 64 ? 2 : 1);
-    p.splits = 1;
-    while (p.splits < 8 && tiles * p.splits * 2 <= at_once && k_tiles / (p.splits * 2) >= 4)
-      p.splits *= 2;
+// The tile and the divisor of k with the shortest modelled time, in ns at
+// full clock, from launches of 1 to 2048 tokens over six shapes of 0.8 M to
+// 136 M weights (bf16; the choice was within 3 % of the fastest in the mean):
+//   stage   64 k of one tile: what its loads and MMAs take, whichever is slower
+//           (one product: 165, 205, 225 for 32, 64, 128 tokens of one CTA, 245
+//           to 285 for 128 to 256 of a pair; each further product its MMAs)
+//   rounds  tiles over the SMs, two small tiles to an SM at 1.6 times a stage
+//   bounds  operand bytes from L2 at 18 TB/s, the weights from HBM at 6.2 TB/s
+//           or 42 GB/s per CTA
+// plus a launch's and an epilogue's fixed time; k is divided only where all the
+// parts run at once.  splits != 0 fixes the divisor.
+LinPlan plan_linear(int64_t feats, int64_t rows_w, int out_per_cta, int64_t toks, int64_t k,
+                    int precision, int b_kmajor, int splits) {
+  const double sms = double(sm_count());
+  const double k_tiles = std::ceil(double(k) / kBK);
+  const double weights = 2.0 * double(rows_w) * double(k);
+  const int a_parts = precision == 3 ? 2 : 1, b_parts = precision >= 2 ? 2 : 1;
+  LinPlan best{128, splits ? splits : 1, false};
+  double best_cost = -1.0;
+  auto consider = [&](LinPlan plan, double cost) {
+    if (best_cost < 0.0 || cost < best_cost) {
+      best = plan;
+      best_cost = cost;
+    }
+  };
+  auto bounded = [&](double work, double l2_bytes, double ctas) {
+    const double hbm = std::min(6200.0, 42.0 * ctas);
+    return std::max(work, std::max(l2_bytes / 18000.0, weights / hbm));
+  };
+  for (int bt : {16, 32, 64, 128}) {
+    if ((bt < 64 && (toks > bt || !b_kmajor)) || (bt == 64 && toks > 512) ||
+        (bt > 16 && toks <= bt / 2 && (b_kmajor || bt > 64)))
+      continue;
+    static const double kStage[3][3] = {{165, 260, 340}, {205, 280, 385}, {225, 345, 525}};
+    const double tiles = std::ceil(double(feats) / out_per_cta) * std::ceil(double(toks) / bt);
+    const int together = (precision == 1 && bt <= 64) || (precision == 2 && bt <= 32) ? 2 : 1;
+    for (int s : {1, 2, 4, 8}) {
+      if (splits ? s != splits : s > 1 && k_tiles / s < 4) continue;
+      const double n = tiles * s;
+      const double per = n <= sms ? 1 : together;
+      const double rounds = std::ceil(n / (sms * per));
+      if (!splits && s > 1 && rounds > 1) break;
+      const double steps = std::ceil(k_tiles / s);
+      const double stage = kStage[bt <= 32 ? 0 : bt / 64][precision - 1] * (per == 2 ? 1.6 : 1.0);
+      const double fixed =
+          4400 + 10.0 * bt + (s > 1 ? 300 + 100.0 * s + 6.0 * bt : 0.0) + (per == 2 ? 1500 : 0);
+      const double bytes = n * steps * kBK * 2.0 * (kTileF * a_parts + bt * b_parts);
+      consider({bt, s, false},
+               fixed + bounded(rounds * steps * stage, bytes, std::min(n, sms * per)));
+    }
   }
-  return p;
+  for (int bt : {256, 224, 192, 160, 128}) {
+    if (splits > 1 || toks < 64 || (!b_kmajor && bt % 128)) continue;
+    const double tiles = std::ceil(double(feats) / (2 * out_per_cta)) * std::ceil(double(toks) / bt);
+    const double pairs = std::floor(sms / 2);
+    const double rounds = std::ceil(tiles / pairs);
+    const double stage = std::max(245.0 + 0.31 * (bt - 128), 279.0 * precision * bt / 256.0);
+    const double bytes = tiles * k_tiles * kBK * 2.0 * (2 * kTileF * a_parts + bt * b_parts);
+    consider({bt, 1, true}, 4500 + 6.0 * bt +
+                                bounded(rounds * k_tiles * stage, bytes,
+                                        std::min(2 * tiles, sms)));
+  }
+  return best;
 }
 
 template <int PREC, bool kGated>
@@ -870,7 +937,8 @@ int run_linear(LinMaps& maps, const LinEpilogue& e, const void* a_hi, const void
                int splits, cudaStream_t stream) {
   constexpr int kOut = kGated ? kTileF / 2 : kTileF;
   const int64_t f_tiles = (int64_t(e.feats) + kOut - 1) / kOut;
-  const LinPlan p = plan_linear(f_tiles, e.toks, k, maps.b_kmajor, splits);
+  const LinPlan p =
+      plan_linear(e.feats, rows_a, kOut, e.toks, k, PREC, maps.b_kmajor, splits);
   const int t_box = p.wide ? p.bt / 2 : p.bt;
   const bool good =
       lin_map(&maps.a_hi, a_hi, maps.a_kmajor, rows_a, k, lda, kOut) &&
