@@ -614,7 +614,7 @@ int mr_topk_logits(const void* logits, int64_t rows, int n, int64_t ld, int k, i
  * gives NaN in that row.  weight NULL: 1.  logits (rows, n), row stride ld, of
  * `dtype`.  Outputs, any may be NULL: loss float32 (rows); the gradient either
  * as `dtype` in grad (may be logits itself, with ldg = ld) or as a bf16 pair
- * grad_hi / grad_lo, row stride ldg.  1 <= k <= 256.
+ * grad_hi / grad_lo, row stride ldg.  1 <= k <= 256, 1e-3 <= temperature <= 1e3.
  */
 int mr_distill_topk(const void* logits, int64_t rows, int n, int64_t ld, int dtype,
                     const float* t_logits, const int64_t* t_index, int k, double temperature,
@@ -665,9 +665,9 @@ int mr_linear(const mr_linear_operand* x, const mr_linear_operand* w, int64_t to
               float* pre, int64_t ldp, int splits, void* stream);
 
 /*
- * The element-wise part of K13's backward: dz = dy * act'(z) as a bf16 pair
- * (toks, feats; twice as many columns [gate | up] under SwiGLU), row stride
- * ldo, the operand of the gradient products mr_linear forms from it (dx = dz w,
+ * The element-wise part of K13's backward: dz = dy * act'(z) in bf16 (hi), or as
+ * a pair with lo (NULL: hi alone), (toks, feats; twice as many columns
+ * [gate | up] under SwiGLU), row stride ldo, the operand of the gradient products mr_linear forms from it (dx = dz w,
  * dw = dz^T x), and bias_grad = sum over tokens of dz (float32, or NULL).  dy
  * MR_F32 or MR_BF16, z the `pre` of mr_linear (NULL where act is none).  The bias gradient needs a
  * workspace of mr_act_grad_workspace_bytes, which must not be shared by calls

@@ -1,7 +1,8 @@
-// The element-wise part of K13's backward: dz = dy act'(z) as a bf16 hi/lo pair
-// (the operand of the two gradient products), and the bias gradient sum_t dz.
+// The element-wise part of K13's backward: dz = dy act'(z) in bf16 or as a bf16
+// hi/lo pair (the operand of the two gradient products), and the bias gradient
+// sum_t dz.
 //
-// HBM-bound: z (float32) and dy are read once, the pair is written once.  A
+// HBM-bound: z (float32) and dy are read once, dz is written once.  A
 // block takes a strip of 256 features and 64 tokens: 64 threads of four
 // features by four token lanes.  Bias sums stay in float32 registers, are
 // joined in the block and written per strip; a second kernel adds the strips
@@ -63,11 +64,12 @@ __device__ __forceinline__ void put_pair(uint16_t* hi, uint16_t* lo, int64_t at,
   if constexpr (V == 4) {
     *reinterpret_cast<uint2*>(hi + at) = make_uint2(uint32_t(h[0]) | (uint32_t(h[1]) << 16),
                                                     uint32_t(h[2]) | (uint32_t(h[3]) << 16));
-    *reinterpret_cast<uint2*>(lo + at) = make_uint2(uint32_t(l[0]) | (uint32_t(l[1]) << 16),
+    if (lo)
+      *reinterpret_cast<uint2*>(lo + at) = make_uint2(uint32_t(l[0]) | (uint32_t(l[1]) << 16),
                                                     uint32_t(l[2]) | (uint32_t(l[3]) << 16));
   } else {
     hi[at] = h[0];
-    lo[at] = l[0];
+    if (lo) lo[at] = l[0];
   }
 }
 
@@ -170,7 +172,7 @@ extern "C" int mr_act_grad(const void* dy, int dy_dtype, int64_t ldy, const floa
                            int64_t toks, int64_t feats, int act, uint16_t* hi, uint16_t* lo,
                            int64_t ldo, float* bias_grad, void* workspace, void* stream) {
   const int rows = act == MR_ACT_SWIGLU ? 2 : 1;
-  if (!dy || (!z && act != MR_ACT_NONE) || !hi || !lo || toks <= 0 || feats <= 0 || feats > 0x3fffffff ||
+  if (!dy || (!z && act != MR_ACT_NONE) || !hi || toks <= 0 || feats <= 0 || feats > 0x3fffffff ||
       act < MR_ACT_NONE || act > MR_ACT_SWIGLU || ldy < feats || (z && ldz < rows * feats) ||
       ldo < rows * feats || (dy_dtype != MR_F32 && dy_dtype != MR_BF16) ||
       strips_of(toks) > 65535)

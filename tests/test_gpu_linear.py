@@ -226,7 +226,10 @@ def test_gradients(K, act, T, F, k):
             lost = 2.0 ** -16 if kind == 3 else 0.0
             off = (ea @ b.abs() + ((products * (n / 16 + 1) + 16) * 2.0 ** -23 + lost) * 1.01 * mass)
             close(got, ref, off, 2.0 ** -24)
-            close(got16, ref, off, 2.0 ** -8)
+            # bf16 gradients of single operands: dz is rounded to bf16 first, by at
+            # most 2**-8 |dz|, hence by 2**-8 sum |dz| |b| in the product
+            rounded = 2.0 ** -8 if kind == 1 else 0.0
+            close(got16, ref, off + rounded * mass, 2.0 ** -8)
         ref = dz.sum(0)
         off = 2.0 ** -19 * size.sum(0) + (T / 4 + 8) * 2.0 ** -24 * dz.abs().sum(0)
         close(db, ref, off, 2.0 ** -24)
