@@ -1,8 +1,9 @@
 """Decoder architectures of the benchmark configurations.
 
 Llama (SmolLM2) and Qwen2 decoder layers as mlx-lm builds them: RMSNorm,
-q/k/v projections (Qwen2 with bias), rotary embedding over the full head
-dimension in the non-interleaved ("rotate half") form, causal grouped-query
+q/k/v projections (Qwen2 with bias), rotary embedding, by default over the full
+head dimension in the non-interleaved ("rotate half") form, its frequencies
+scaled for long contexts where the architecture says so, causal grouped-query
 attention with scale ``head_dim ** -0.5``, output projection, residual,
 RMSNorm, SwiGLU MLP, residual.  The reference runs the mlx-lm layer inside
 ``block_output`` (mround/pipeline/blocks.py:578-606); its math is restated in
@@ -13,7 +14,48 @@ from __future__ import annotations
 
 import dataclasses
 
-__all__ = ["ARCHITECTURES", "Arch", "get_arch"]
+__all__ = ["ARCHITECTURES", "Arch", "RopeScaling", "get_arch"]
+
+ROPE_SCALINGS = ("linear", "llama3", "yarn")
+
+
+@dataclasses.dataclass(frozen=True, slots=True)
+class RopeScaling:
+    """How rotary frequencies are scaled for contexts longer than trained on.
+
+    ``kind`` "linear": every frequency divided by ``factor``.  "llama3":
+    wavelengths above ``original_max_position / low_freq_factor`` divided by
+    ``factor``, those below ``original_max_position / high_freq_factor`` kept,
+    a ramp in between.  "yarn": frequencies that turn fewer than ``beta_slow``
+    times in ``original_max_position`` positions divided, more than
+    ``beta_fast`` kept, a ramp over the columns in between, and cosines and
+    sines multiplied by ``attention_factor`` (0.1 ln(factor) + 1 when None)."""
+
+    kind: str
+    factor: float
+    original_max_position: int | None = None
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: float | None = None
+
+    def __post_init__(self) -> None:
+        from mround_b200.exceptions import ArchitectureError
+
+        if self.kind not in ROPE_SCALINGS:
+            raise ArchitectureError(f"rope scaling {self.kind!r} is not one of "
+                                    f"{', '.join(ROPE_SCALINGS)}")
+        if not self.factor >= 1.0:
+            raise ArchitectureError(f"rope scaling factor must be at least 1, got {self.factor}")
+        if self.kind != "linear" and not (self.original_max_position or 0) > 0:
+            raise ArchitectureError(f"{self.kind} rope scaling needs the original number of "
+                                    "positions")
+        if self.kind == "llama3" and not 0 < self.low_freq_factor < self.high_freq_factor:
+            raise ArchitectureError("llama3 rope scaling needs 0 < low_freq_factor < "
+                                    "high_freq_factor")
+        if self.kind == "yarn" and not 0 < self.beta_slow < self.beta_fast:
+            raise ArchitectureError("yarn rope scaling needs 0 < beta_slow < beta_fast")
 
 
 @dataclasses.dataclass(frozen=True, slots=True)
@@ -31,6 +73,21 @@ class Arch:
     rope_theta: float
     qkv_bias: bool
     tied: bool
+    rope_scaling: RopeScaling | None = None
+    rope_interleaved: bool = False  # pairs (2j, 2j + 1) instead of halves
+    rotary_dim: int | None = None  # rotated columns of a head; all of them when None
+
+    def __post_init__(self) -> None:
+        r = self.rotary_dim
+        if r is not None and (r % 2 or not 2 <= r <= self.head_dim):
+            from mround_b200.exceptions import ArchitectureError
+
+            raise ArchitectureError(f"rotary_dim must be even and at most the head dimension "
+                                    f"{self.head_dim}, got {r}")
+
+    @property
+    def rope_layout(self) -> str:
+        return "interleaved" if self.rope_interleaved else "half"
 
     @property
     def q_dim(self) -> int:

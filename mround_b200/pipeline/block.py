@@ -4,8 +4,8 @@ The block is the mlx-lm Llama/Qwen2 decoder layer the reference runs in
 ``block_output`` (mround/pipeline/blocks.py:578-606), in float32 semantics.
 The tuning path (``forward_fused`` / ``backward_fused``) runs every op on this
 library's kernels -- the linears and the attention products on the tcgen05
-GEMM (K3), norms, RoPE, softmax and SwiGLU on K7 -- with an explicit
-backward; ``DeviceBlock.forward`` is an autograd form (K3 linears, torch for
+GEMMs (K3; K13 where a residual or SwiGLU follows), norms, RoPE, softmax and
+SwiGLU's backward on K7 -- with an explicit backward; ``DeviceBlock.forward`` is an autograd form (K3 linears, torch for
 the rest) kept as a cross-check:
 
     h1  = rmsnorm(x) * w_in            q|k|v = h1 @ Wqkv^T (+ b)
@@ -36,7 +36,7 @@ import torch
 import torch.nn.functional as F
 
 from mround_b200 import kernels
-from mround_b200.pipeline.arch import Arch
+from mround_b200.pipeline.arch import Arch, RopeScaling
 from mround_b200.pipeline.attention import attention
 from mround_b200.pipeline.model import BlockParams
 
@@ -210,19 +210,56 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
     return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * w.float()
 
 
-def rope_tables(seq_len: int, head_dim: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
-    """cos/sin (seq_len, head_dim/2) of the non-interleaved rotary embedding."""
+def rope_tables(seq_len: int, head_dim: int, theta: float, device,
+                scaling: RopeScaling | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """float32 cos/sin (seq_len, head_dim/2) of the rotary embedding over
+    ``head_dim`` columns, angles in float64."""
     half = head_dim // 2
     inv = theta ** (-torch.arange(0, half, dtype=torch.float64, device=device) * 2.0 / head_dim)
+    scale = 1.0
+    if scaling is not None:
+        inv, scale = _scaled_frequencies(inv, head_dim, theta, scaling)
     ang = torch.arange(seq_len, dtype=torch.float64, device=device)[:, None] * inv[None, :]
-    return torch.cos(ang).float(), torch.sin(ang).float()
+    return (torch.cos(ang) * scale).float(), (torch.sin(ang) * scale).float()
 
 
-def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
-    """x (B, H, S, D): rotate the two halves of each head vector."""
-    half = x.shape[-1] // 2
-    x1, x2 = x[..., :half], x[..., half:]
-    return torch.cat((x1 * cos - x2 * sin, x1 * sin + x2 * cos), dim=-1)
+def _scaled_frequencies(inv, dim: int, theta: float, s: RopeScaling):
+    """(frequencies, factor on cosines and sines) under a :class:`RopeScaling`."""
+    if s.kind == "linear":
+        return inv / s.factor, 1.0
+    original = float(s.original_max_position)
+    if s.kind == "llama3":
+        turns = original * inv / (2.0 * math.pi)  # in the original context
+        keep = ((turns - s.low_freq_factor) / (s.high_freq_factor - s.low_freq_factor)).clamp(0, 1)
+        return inv / s.factor * (1 - keep) + inv * keep, 1.0
+
+    def column(turns: float) -> float:
+        """The pair whose frequency turns so often in the original context."""
+        return dim * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
+
+    low = max(math.floor(column(s.beta_fast)), 0)
+    high = min(math.ceil(column(s.beta_slow)), dim - 1)
+    width = max(high - low, 0.001)
+    pairs = torch.arange(inv.shape[0], dtype=torch.float64, device=inv.device)
+    keep = 1 - ((pairs - low) / width).clamp(0, 1)
+    scale = s.attention_factor
+    if scale is None:
+        scale = 0.1 * math.log(s.factor) + 1.0
+    return inv / s.factor * (1 - keep) + inv * keep, scale
+
+
+def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+               layout: str = "half") -> torch.Tensor:
+    """x (B, H, S, D): rotate the pairs of each head vector's first columns, as
+    many as the tables cover."""
+    half = cos.shape[-1]
+    r = 2 * half
+    if layout == "interleaved":
+        x1, x2 = x[..., 0:r:2], x[..., 1:r:2]
+        turned = torch.stack((x1 * cos - x2 * sin, x1 * sin + x2 * cos), dim=-1).flatten(-2)
+        return torch.cat((turned, x[..., r:]), dim=-1)
+    x1, x2 = x[..., :half], x[..., half:r]
+    return torch.cat((x1 * cos - x2 * sin, x1 * sin + x2 * cos, x[..., r:]), dim=-1)
 
 
 class DeviceBlock:
@@ -255,8 +292,9 @@ class DeviceBlock:
 
     def _tables(self, seq_len: int):
         if seq_len not in self._rope:
-            self._rope[seq_len] = rope_tables(seq_len, self.arch.head_dim, self.arch.rope_theta,
-                                              self.device)
+            a = self.arch
+            self._rope[seq_len] = rope_tables(seq_len, a.rotary_dim or a.head_dim, a.rope_theta,
+                                              self.device, a.rope_scaling)
         return self._rope[seq_len]
 
     def forward(self, x: torch.Tensor, prec: Precision, *, train: bool = False) -> torch.Tensor:
@@ -272,8 +310,8 @@ class DeviceBlock:
         k = k.view(b, s, a.kv_heads, a.head_dim).transpose(1, 2)
         v = v.view(b, s, a.kv_heads, a.head_dim).transpose(1, 2)
         cos, sin = self._tables(s)
-        q = apply_rope(q, cos, sin)
-        k = apply_rope(k, cos, sin)
+        q = apply_rope(q, cos, sin, a.rope_layout)
+        k = apply_rope(k, cos, sin, a.rope_layout)
         att = attention(q, k, v, 1.0 / math.sqrt(a.head_dim))
         att = att.transpose(1, 2).reshape(b, s, a.q_dim)
         h = x + lin("o", att)
@@ -287,9 +325,9 @@ class DeviceBlock:
 # Explicit fused path: the same block, forward and backward written out.
 #
 # Every element-wise step is one kernel that writes the next GEMM operand as
-# bf16 hi/lo (csrc/blockops.cu); the residual additions are folded into the
-# GEMMs (C is preloaded with the residual and accumulated into); the backward
-# never forms the block-input gradient, which the tuning step does not need.
+# bf16 hi/lo (csrc/blockops.cu); the residual additions and SwiGLU are in their
+# GEMMs' epilogues (K13); the backward never forms the block-input gradient,
+# which the tuning step does not need.
 # Saved for the backward: the operand splits, P (float32 and hi/lo), h, gu,
 # and the second norm's rstd.
 
@@ -309,6 +347,16 @@ def _wprec(layer: FusedLinear, want: int) -> int:
     if want == TF32:
         return TF32
     return want if layer.wq_lo is not None else min(want, 2)
+
+
+def _linear(layer: FusedLinear, x, want: int, **epilogue):
+    """A linear of ``x`` (hi, lo, ...) on K13 with what follows it in its
+    epilogue.  ``splits=1``: a token's output does not depend on how many
+    tokens the call has, and adds up in K3's order."""
+    prec = _wprec(layer, want)
+    return kernels.linear((x[0], x[1]) if prec >= 2 else x[0],
+                          (layer.wq_hi, layer.wq_lo) if prec == 3 else layer.wq_hi,
+                          splits=1, **epilogue)
 
 
 def _fused_forward(self: DeviceBlock, x: torch.Tensor, prec: Precision, save: bool,
@@ -337,13 +385,11 @@ def _fused_forward(self: DeviceBlock, x: torch.Tensor, prec: Precision, save: bo
     h1 = (h1_hi, h1_lo, h1_t)
     qkv_l = L["qkv"]
     stats("qkv", h1)
-    L["qkv"].ready()
-    qkv = torch.empty((t, qkv_l.out_features), dtype=torch.float32, device=x.device)
-    p = _wprec(qkv_l, prec.forward)
-    _mm(h1, (qkv_l.wq_hi, qkv_l.wq_lo), qkv, m=t, n=qkv_l.out_features, k=h, a_kmajor=True,
-        b_kmajor=True, lda=h, ldb=h, prec=p, bias=qkv_l.bias)
+    qkv_l.ready()
+    qkv = _linear(qkv_l, h1, prec.forward, bias=qkv_l.bias, dtype=torch.float32)
     cos, sin = self._tables(s)
-    q, k, v = kernels.rope_split(qkv, cos, sin, b, s, hq, hkv, d)
+    q, k, v = kernels.rope_split(qkv, cos, sin, b, s, hq, hkv, d, layout=a.rope_layout,
+                                 rotary_dim=a.rotary_dim)
     del qkv
     band = s % 128 == 0  # causal tile skipping needs 128-aligned heads
     c1, c2 = (1, 2) if band else (0, 0)
@@ -360,23 +406,20 @@ def _fused_forward(self: DeviceBlock, x: torch.Tensor, prec: Precision, save: bo
     o_l = L["o"]
     stats("o", att)
     o_l.ready()
-    hres = x2.clone()
-    _mm(att, (o_l.wq_hi, o_l.wq_lo), hres, m=t, n=h, k=hq * d, a_kmajor=True, b_kmajor=True,
-        lda=hq * d, ldb=hq * d, prec=_wprec(o_l, prec.forward), accumulate=True)
+    hres = _linear(o_l, att, prec.forward, residual=x2, dtype=torch.float32)
     h2_hi, h2_lo, rstd2, h2_t = kernels.rmsnorm_split(hres, self.post_norm, a.rms_eps, t32=t32)
     gu_l = L["gate_up"]
     stats("gate_up", (h2_hi, h2_lo))
     gu_l.ready()
-    gu = torch.empty((t, 2 * inter), dtype=torch.float32, device=x.device)
-    _mm((h2_hi, h2_lo), (gu_l.wq_hi, gu_l.wq_lo), gu, m=t, n=2 * inter, k=h, a_kmajor=True,
-        b_kmajor=True, lda=h, ldb=h, prec=_wprec(gu_l, prec.forward))
-    act = kernels.swiglu_split(gu, t, inter, t32=t32)
+    # the backward reads gate|up; without one they never leave the epilogue
+    gu = torch.empty((t, 2 * inter), dtype=torch.float32, device=x.device) if save else None
+    act_t = torch.empty((t, inter), dtype=torch.float32, device=x.device) if t32 else None
+    act = (*_linear(gu_l, (h2_hi, h2_lo), prec.forward, act="swiglu", split=True, pre=gu,
+                    t32=act_t), act_t)
     dn_l = L["down"]
     stats("down", act)
     dn_l.ready()
-    out = hres.clone()
-    _mm(act, (dn_l.wq_hi, dn_l.wq_lo), out, m=t, n=h, k=inter, a_kmajor=True, b_kmajor=True,
-        lda=inter, ldb=inter, prec=_wprec(dn_l, prec.forward), accumulate=True)
+    out = _linear(dn_l, act, prec.forward, residual=hres, dtype=torch.float32)
     saved = None
     if save:
         saved = dict(shape=(b, s, h), h1=h1, q=q, k=k, v=v, probs=probs, att=att, hres=hres,
@@ -489,7 +532,7 @@ def _fused_backward(self: DeviceBlock, saved: dict, dout: torch.Tensor, prec: Pr
     del g_s
     cos, sin = self._tables(s)
     g_qkv = kernels.rope_bwd_split(dq, dk, dv, cos, sin, b, s, hq, hkv, d, split=need_split,
-                                   t32=need_t32)
+                                   t32=need_t32, layout=a.rope_layout, rotary_dim=a.rotary_dim)
     del dq, dk, dv
     weight_grad(qkv_l, g_qkv, saved["h1"], qkv_l.out_features, h)
     if not want_dx:

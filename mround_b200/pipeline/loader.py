@@ -12,8 +12,9 @@ lazy load does, and served through the same interface as
 Refused loudly, as the reference refuses (loader.py:245-254) or because the
 device path does not implement them: a checkpoint that is already quantized
 (``quantization`` / ``quantization_config`` in its configuration), a model type
-other than ``llama`` / ``qwen2``, RoPE scaling, and block linears not stored
-in bf16 (the tuning kernels read bf16 weights; converting fp16 or fp32 weights
+other than ``llama`` / ``qwen2``, RoPE scaling of another kind than linear,
+llama3 and yarn or without its parameters, and block linears not stored in
+bf16 (the tuning kernels read bf16 weights; converting fp16 or fp32 weights
 would change the model being quantized).
 """
 
@@ -27,7 +28,7 @@ import numpy as np
 import torch
 
 from mround_b200.exceptions import ArchitectureError
-from mround_b200.pipeline.arch import Arch
+from mround_b200.pipeline.arch import Arch, RopeScaling
 from mround_b200.pipeline.model import BlockParams
 
 __all__ = ["CheckpointModel", "is_checkpoint_dir"]
@@ -40,6 +41,49 @@ _LINEARS = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_at
 def is_checkpoint_dir(path: str | Path) -> bool:
     p = Path(path)
     return p.is_dir() and (p / "config.json").is_file()
+
+
+# what each scaling's configuration has to state, and may state
+_ROPE_KEYS = {
+    "linear": (("factor",), ()),
+    "llama3": (("factor", "low_freq_factor", "high_freq_factor",
+                "original_max_position_embeddings"), ()),
+    "yarn": (("factor", "original_max_position_embeddings"),
+             ("beta_fast", "beta_slow", "attention_factor")),
+}
+
+
+def _rope_scaling(where: str, entry) -> RopeScaling | None:
+    """The scaling that a configuration's ``rope_scaling`` or ``rope_parameters``
+    describes; None for the unscaled embedding.  Refused: a kind this block does
+    not compute, a key it would ignore, or a missing one (readers disagree on
+    defaults)."""
+    if not entry:
+        return None
+    kind = entry.get("rope_type", entry.get("type", "default"))
+    said = f"{where} {entry} (rope_type {kind!r})"
+    if kind == "default":
+        return None
+    if kind not in _ROPE_KEYS:
+        raise ArchitectureError(f"{said} is not implemented by the device block")
+    needed, optional = _ROPE_KEYS[kind]
+    missing = [k for k in needed if entry.get(k) is None]
+    if missing:
+        raise ArchitectureError(f"{said} does not state {', '.join(missing)}")
+    known = {"rope_type", "type", "rope_theta", "original_max_position_embeddings", *needed,
+             *optional}
+    # settings whose stated value is what the block does
+    same = {"partial_rotary_factor": 1.0, "truncate": True}
+    unknown = sorted(k for k, v in entry.items()
+                     if k not in known and v is not None and v != same.get(k))
+    if unknown:
+        raise ArchitectureError(f"{said}: {', '.join(unknown)} is not implemented by the device "
+                                "block")
+    given = {k: float(entry[k]) for k in (*needed, *optional)
+             if k != "original_max_position_embeddings" and entry.get(k) is not None}
+    original = entry.get("original_max_position_embeddings")
+    return RopeScaling(kind, original_max_position=None if original is None else int(original),
+                       **given)
 
 
 class _SafetensorsFile:
@@ -89,9 +133,6 @@ class CheckpointModel:
         if family not in ("llama", "qwen2"):
             raise ArchitectureError(f"model_type {family!r} is not supported; the B200 path "
                                     "implements the llama and qwen2 decoder layers")
-        if config.get("rope_scaling"):
-            raise ArchitectureError(f"rope_scaling {config['rope_scaling']} is not implemented "
-                                    "by the device block")
         if config.get("use_sliding_window"):
             raise ArchitectureError(f"use_sliding_window with sliding_window="
                                     f"{config.get('sliding_window')} is not implemented by the "
@@ -108,10 +149,9 @@ class CheckpointModel:
         # transformers >= 5 writes the rotary settings as ``rope_parameters``
         # ({"rope_type", "rope_theta", ...}) instead of top-level keys
         rope = config.get("rope_parameters") or {}
-        if rope.get("rope_type", "default") != "default":
-            raise ArchitectureError(f"rope_parameters {rope} (rope_type "
-                                    f"{rope.get('rope_type')!r}) is not implemented by the "
-                                    "device block")
+        scaling = _rope_scaling("rope_scaling", config.get("rope_scaling"))
+        if scaling is None:
+            scaling = _rope_scaling("rope_parameters", rope)
         theta = config.get("rope_theta")
         if theta is None:
             theta = rope.get("rope_theta", 10000.0)
@@ -127,7 +167,9 @@ class CheckpointModel:
             rms_eps=float(config.get("rms_norm_eps", 1e-6)),
             rope_theta=float(theta),
             qkv_bias=family == "qwen2",
-            tied=bool(config.get("tie_word_embeddings", False)))
+            tied=bool(config.get("tie_word_embeddings", False)),
+            rope_scaling=scaling,
+            rope_interleaved=bool(config.get("rope_traditional", False)))
         self._files: dict[str, _SafetensorsFile] = {}
         self._where: dict[str, str] = {}
         index = self.path / "model.safetensors.index.json"

@@ -21,7 +21,7 @@ import hashlib
 import numpy as np
 import torch
 
-from mround_b200.pipeline.arch import Arch
+from mround_b200.pipeline.arch import Arch, RopeScaling
 
 __all__ = ["BlockParams", "SyntheticModel", "zipf_tokens", "tensor_seed"]
 
@@ -105,6 +105,13 @@ class SyntheticModel:
 
     def config(self) -> dict:
         a = self.arch
+        rope = {}
+        if a.rope_scaling is not None:
+            rope["rope_scaling"] = rope_scaling_config(a.rope_scaling)
+        if a.rope_interleaved:
+            rope["rope_traditional"] = True
+        if a.rotary_dim is not None:
+            rope["partial_rotary_factor"] = a.rotary_dim / a.head_dim
         return {
             "model_type": a.family,
             "hidden_size": a.hidden,
@@ -118,7 +125,22 @@ class SyntheticModel:
             "rope_theta": a.rope_theta,
             "tie_word_embeddings": a.tied,
             "torch_dtype": "bfloat16",
+            **rope,
         }
+
+
+def rope_scaling_config(s: RopeScaling) -> dict:
+    """The ``rope_scaling`` entry of a checkpoint configuration."""
+    entry: dict = {"rope_type": s.kind, "factor": s.factor}
+    if s.original_max_position is not None:
+        entry["original_max_position_embeddings"] = s.original_max_position
+    if s.kind == "llama3":
+        entry.update(low_freq_factor=s.low_freq_factor, high_freq_factor=s.high_freq_factor)
+    if s.kind == "yarn":
+        entry.update(beta_fast=s.beta_fast, beta_slow=s.beta_slow)
+        if s.attention_factor is not None:
+            entry["attention_factor"] = s.attention_factor
+    return entry
 
 
 def zipf_tokens(vocab: int, n_samples: int, seq_len: int, seed: int = 42, s: float = 1.1) -> np.ndarray:

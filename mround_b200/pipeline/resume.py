@@ -67,6 +67,17 @@ def _scheme_dict(scheme: QuantScheme) -> dict[str, Any]:
             "symmetry": scheme.symmetry.value, "scale_init": scheme.scale_init.value}
 
 
+def _arch_dict(arch: Any) -> Any:
+    """The architecture's fields; optional ones only where they are set, so that
+    a directory written before a field existed stays valid."""
+    if not dataclasses.is_dataclass(arch):
+        return str(arch)
+    optional = {f.name: f.default for f in dataclasses.fields(arch)
+                if f.default is not dataclasses.MISSING}
+    return {k: v for k, v in dataclasses.asdict(arch).items()
+            if k not in optional or v != optional[k]}
+
+
 def run_fingerprint(*, model: str, arch: Any, scheme: QuantScheme, tuning: Any,
                     scheme_by_layer: Mapping[str, QuantScheme] | None, batches: Sequence[Any],
                     world: int, **extra: Any) -> dict[str, Any]:
@@ -77,7 +88,7 @@ def run_fingerprint(*, model: str, arch: Any, scheme: QuantScheme, tuning: Any,
     return {
         "format": FORMAT,
         "model": str(model),
-        "arch": dataclasses.asdict(arch) if dataclasses.is_dataclass(arch) else str(arch),
+        "arch": _arch_dict(arch),
         "scheme": _scheme_dict(scheme),
         "scheme_by_layer": overrides,
         "tuning": dataclasses.asdict(tuning) if dataclasses.is_dataclass(tuning) else str(tuning),
