@@ -180,7 +180,8 @@ def _rtn_layer(weight: torch.Tensor, scheme: QuantScheme, device) -> QuantizedLa
 
 
 def _plan_mixed(model, resolved, average_bits, candidate_bits, *, gradient_source, scoring_samples,
-                scoring_seq_len, scoring_batch_size, seed, device, given_plan=None, dist=None):
+                scoring_seq_len, scoring_batch_size, seed, device, given_plan=None, dist=None,
+                objective="labels", top_logits=64, temperature=1.0):
     from mround_b200.pipeline.scoring import score_widths
     from mround_b200.planner.allocator import allocate_bits
     from mround_b200.planner.sensitivity import (
@@ -208,7 +209,8 @@ def _plan_mixed(model, resolved, average_bits, candidate_bits, *, gradient_sourc
     tokens = zipf_tokens(arch.vocab, n, s, seed=DEFAULT_SEED if seed is None else seed)
     batches = [tokens[i:i + bsz] for i in range(0, n - bsz + 1, bsz)]
     scored = score_widths(model, batches, widths, resolved, gradient_source=source, device=device,
-                          dist=dist)
+                          dist=dist, objective=objective, top_logits=top_logits,
+                          temperature=temperature)
     budget = mixed_budget_bits(scored.shapes, average_bits, resolved.group_size)
     options = score_layer_options(scored.scores, scored.shapes, resolved)
     alloc = allocate_bits(options, budget_bits=budget)
@@ -222,6 +224,9 @@ def _plan_mixed(model, resolved, average_bits, candidate_bits, *, gradient_sourc
         "describe": (f"mixed plan: {alloc.average_bits:.3f} bits average over "
                      f"{len(alloc.by_layer)} layers, scored in {scored.seconds:.1f}s ({source})"),
     }
+    if objective != "labels":
+        info["objective"] = {"name": objective, "top_logits": top_logits,
+                             "temperature": temperature, "losses": scored.losses}
     return overrides, info
 
 
@@ -268,15 +273,35 @@ def quantize(model: str | Path | SyntheticModel, *, output_dir: str | Path, bits
              min_block_coverage: float = MIN_BLOCK_COVERAGE, seed: int | None = None,
              memory_budget: int | None = None, memory_check: bool = True,
              progress=print, dist: DistContext | None = None,
-             resume_dir: str | Path | None = None) -> QuantizeResult:
+             resume_dir: str | Path | None = None, sensitivity_objective: str = "labels",
+             sensitivity_top_logits: int = 64,
+             sensitivity_temperature: float = 1.0) -> QuantizeResult:
     """Quantize ``model`` and write an MLX checkpoint to ``output_dir``.
 
     ``resume_dir`` (not in the reference): record every finished block there,
     and continue a run that stopped, tuning only the blocks it had not
     finished (:mod:`mround_b200.pipeline.resume`).  A directory written by a
-    run with different settings or calibration is refused."""
+    run with different settings or calibration is refused.
+
+    ``sensitivity_objective`` (not in the reference): what a mixed run's scoring
+    differentiates, the calibration "labels" or the distillation loss against
+    the dense model's ``sensitivity_top_logits`` largest logits ("teacher") at
+    ``sensitivity_temperature``."""
     if export_format != "mlx":
         raise UnsupportedSchemeError(f"export_format {export_format!r} is not available; use 'mlx'")
+    if sensitivity_objective not in ("labels", "teacher"):
+        raise CalibrationError(f"sensitivity_objective must be 'labels' or 'teacher', got "
+                               f"{sensitivity_objective!r}")
+    if sensitivity_objective == "teacher":
+        if average_bits is None or plan is not None:
+            raise CalibrationError("a sensitivity objective belongs to a scored mixed run "
+                                   "(average_bits without a plan)")
+        if not 1 <= sensitivity_top_logits <= 256:
+            raise CalibrationError("sensitivity_top_logits must be 1 to 256, got "
+                                   f"{sensitivity_top_logits}")
+        if not 1e-3 <= sensitivity_temperature <= 1e3:
+            raise CalibrationError("sensitivity_temperature must be 0.001 to 1000, got "
+                                   f"{sensitivity_temperature}")
     if holdout_batches < 0:
         raise CalibrationError(f"holdout_batches must be zero or more, got {holdout_batches}")
     if plan is not None and average_bits is None:
@@ -315,7 +340,8 @@ def quantize(model: str | Path | SyntheticModel, *, output_dir: str | Path, bits
             bundle, resolved, average_bits, candidate_bits, gradient_source=sensitivity_gradients,
             scoring_samples=scoring_samples, scoring_seq_len=scoring_seq_len,
             scoring_batch_size=scoring_batch_size, seed=seed, device=device, given_plan=plan,
-            dist=dist)
+            dist=dist, objective=sensitivity_objective, top_logits=sensitivity_top_logits,
+            temperature=sensitivity_temperature)
         remainder_scheme = resolved.with_bits(_remainder_width(average_bits, candidate_bits,
                                                                remainder_bits))
         plan_info["remainder_bits"] = remainder_scheme.bits

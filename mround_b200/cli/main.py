@@ -62,6 +62,13 @@ def build_parser() -> argparse.ArgumentParser:
                    help="Tokens per scoring sequence (api scoring_seq_len).")
     q.add_argument("--sensitivity-gradients", default="auto",
                    choices=["auto", "own_width", "widest"])
+    q.add_argument("--sensitivity-objective", default="labels", choices=["labels", "teacher"],
+                   help="Score a mixed run by the calibration labels, or by distillation from "
+                        "the dense model's top logits.")
+    q.add_argument("--sensitivity-top-logits", type=int, default=64,
+                   help="Logits kept per position for the teacher objective.")
+    q.add_argument("--sensitivity-temperature", type=float, default=1.0,
+                   help="Temperature of the teacher objective.")
     return parser
 
 
@@ -87,6 +94,9 @@ def _quantize(args: argparse.Namespace) -> int:
                       seed=args.seed, memory_budget=args.memory_budget,
                       scoring_samples=args.scoring_samples, scoring_seq_len=args.scoring_seq_len,
                       sensitivity_gradients=args.sensitivity_gradients,
+                      sensitivity_objective=args.sensitivity_objective,
+                      sensitivity_top_logits=args.sensitivity_top_logits,
+                      sensitivity_temperature=args.sensitivity_temperature,
                       memory_check=not args.skip_memory_check,
                       min_block_coverage=0.0 if args.allow_dense else MIN_BLOCK_COVERAGE,
                       resume_dir=args.resume_dir)

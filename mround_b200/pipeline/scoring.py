@@ -12,8 +12,15 @@ perturbation is ever held beyond its layer.
 
 The backward is the blocks' explicit fused forward/backward (the same K3 GEMMs
 and K7 element-wise kernels as the tuning step, plus the block-input gradient)
-and the LM head on K3; the cross-entropy gradient is formed in place on the
-logits.
+and the LM head on K13 and K3; the gradient on the logits is one row-wise kernel.
+
+The objective is the reference's cross-entropy with the calibration labels, or
+(``objective="teacher"``, no counterpart there) the distillation loss against
+the top logits of a teacher -- by default the model itself with its dense
+weights, whose divergence from the anchored model is what quantization loses;
+labels score the model's own errors too.  The teacher's logits are captured
+once per batch by K11 (``capture_top_logits``), the loss and its gradient are
+K12.
 
 ``own_width`` takes one backward per width at that width's anchors (the
 reference's procedure); ``widest`` one backward at the widest width, scoring
@@ -39,7 +46,9 @@ from mround_b200.pipeline.model import SyntheticModel
 from mround_b200.core.scale_search import search_scales
 from mround_b200.schemes import DEFAULT_EPS_FP32, QuantScheme, ScaleInit, Symmetry
 
-__all__ = ["SensitivityScores", "score_widths"]
+__all__ = ["OBJECTIVES", "SensitivityScores", "capture_top_logits", "score_widths"]
+
+OBJECTIVES = ("labels", "teacher")
 
 
 @dataclasses.dataclass(frozen=True)
@@ -48,6 +57,48 @@ class SensitivityScores:
     shapes: dict[str, tuple[int, int]]
     skipped: tuple[tuple[str, str], ...]
     seconds: float
+    # mean distillation loss at each anchor width (objective "teacher")
+    losses: dict[int, float] | None = None
+
+
+def _padded(tokens: torch.Tensor) -> torch.Tensor:
+    """Input tokens padded at the end to a multiple of 8."""
+    pad = (-tokens.shape[1]) % 8
+    if pad:
+        tokens = torch.cat([tokens, tokens[:, -1:].expand(tokens.shape[0], pad)], dim=1)
+    return tokens
+
+
+def _head_logits(norm, head: torch.Tensor, b: int, s: int) -> torch.Tensor:
+    """float32 logits of the first s positions of b padded sequences, from their
+    normed rows (hi, lo)."""
+    hidden = head.shape[1]
+    rows = tuple(p.view(b, -1, hidden)[:, :s].reshape(b * s, hidden) for p in norm)
+    return kernels.linear(rows, head, dtype=torch.float32, splits=1)
+
+
+def capture_top_logits(model, batches: Sequence[np.ndarray], k: int, *,
+                       device: torch.device | str = "cuda") -> list[tuple[torch.Tensor, torch.Tensor]]:
+    """The ``k`` largest logits and their columns at every scored position of
+    each batch, from the model's dense weights: float32 and int64, (positions,
+    k).  One block is on the device at a time."""
+    dev = torch.device(device)
+    arch = model.arch
+    embed = model.embed_tokens().to(dev)
+    inputs = [torch.as_tensor(batch, dtype=torch.long, device=dev)[:, :-1] for batch in batches]
+    streams = [embed[_padded(inp)].float().contiguous() for inp in inputs]
+    del embed
+    for i in range(arch.layers):
+        blk = DeviceBlock(arch, model.block(i), dev)
+        for j, x in enumerate(streams):
+            streams[j], _ = blk.forward_fused(x, Precision(), False)
+    head = model.lm_head().to(dev).contiguous()
+    norm = model.final_norm().to(dev)
+    found = []
+    for inp, x in zip(inputs, streams):
+        hi, lo, _, _ = kernels.rmsnorm_split(x.view(-1, arch.hidden), norm, arch.rms_eps)
+        found.append(kernels.topk_logits(_head_logits((hi, lo), head, *inp.shape), k))
+    return found
 
 
 def score_widths(model: SyntheticModel, batches: Sequence[np.ndarray], widths: Sequence[int],
@@ -55,8 +106,15 @@ def score_widths(model: SyntheticModel, batches: Sequence[np.ndarray], widths: S
                  eps: float = DEFAULT_EPS_FP32, gradient_source: str = "own_width",
                  progress: Callable[[str], None] | None = None,
                  device: torch.device | str = "cuda",
-                 dist: DistContext | None = None) -> SensitivityScores:
+                 dist: DistContext | None = None, objective: str = "labels",
+                 teacher=None, top_logits: int = 64,
+                 temperature: float = 1.0) -> SensitivityScores:
     """Score every block linear at every width (float64 sums on the device).
+
+    ``objective="teacher"``: the loss is the mean over positions of T^2 KL(p, q)
+    against the ``top_logits`` largest logits of ``teacher`` (a model of the
+    same vocabulary; ``model`` itself with dense weights when None) at
+    ``temperature`` T.
 
     Under data parallelism (``dist`` with several ranks) rank r takes batches
     r, r + N, ...; the per-layer float64 sums are all-reduced, so every rank
@@ -66,15 +124,33 @@ def score_widths(model: SyntheticModel, batches: Sequence[np.ndarray], widths: S
         raise ValueError("no candidate widths to score")
     if gradient_source not in ("own_width", "widest"):
         raise ValueError(f"gradient_source must be 'own_width' or 'widest', got {gradient_source!r}")
+    if objective not in OBJECTIVES:
+        raise ValueError(f"objective must be one of {OBJECTIVES}, got {objective!r}")
+    distills = objective == "teacher"
+    if teacher is not None and not distills:
+        raise ValueError("a teacher belongs to objective 'teacher'")
     started = time.perf_counter()
     dev = torch.device(device)
     arch = model.arch
+    if distills:
+        teacher = model if teacher is None else teacher
+        if teacher.arch.vocab != arch.vocab:
+            raise ValueError(f"the teacher's vocabulary has {teacher.arch.vocab} tokens, the "
+                             f"model's {arch.vocab}")
+        if not 1 <= top_logits <= min(arch.vocab, kernels.MAX_TOPK):
+            raise ValueError(f"top_logits must be 1 to {min(arch.vocab, kernels.MAX_TOPK)}, got "
+                             f"{top_logits}")
     if expected_blocks is not None and expected_blocks != arch.layers:
         from mround_b200.exceptions import ArchitectureError
 
         raise ArchitectureError(f"found {arch.layers} blocks but the configuration says {expected_blocks}")
     group = base_scheme.group_size
     widths = sorted(int(w) for w in widths)
+    dist = dist or DistContext()
+    mine = list(batches)[dist.rank::dist.world]
+    targets = [None] * len(mine)
+    if distills:
+        targets = capture_top_logits(teacher, mine, top_logits, device=dev)
     prec = Precision()
     blocks = [DeviceBlock(arch, model.block(i), dev) for i in range(arch.layers)]
     shapes, skipped, paths_by_layer = {}, [], {}
@@ -160,17 +236,16 @@ def score_widths(model: SyntheticModel, batches: Sequence[np.ndarray], widths: S
 
     hidden = arch.hidden
 
-    def backward_pass(batch: np.ndarray) -> None:
-        """Mean shifted cross-entropy of one batch, backward through every block
+    def backward_pass(batch: np.ndarray, target, loss: torch.Tensor) -> None:
+        """One batch's mean loss (shifted cross-entropy, or distillation from
+        ``target``, then added to ``loss``), backward through every block
         (explicit fused forward/backward; each block's weight-gradient GEMMs run
         the K6 hooks)."""
         tokens = torch.as_tensor(batch, dtype=torch.long, device=dev)
         inp, labels = tokens[:, :-1], tokens[:, 1:]
         b, s = inp.shape
-        pad = (-s) % 8
-        if pad:
-            inp = torch.cat([inp, inp[:, -1:].expand(b, pad)], dim=1)
-        sp = s + pad
+        inp = _padded(inp)
+        sp = inp.shape[1]
         x = embed[inp].float().contiguous()
         saved_all = []
         for blk in blocks:
@@ -179,14 +254,16 @@ def score_widths(model: SyntheticModel, batches: Sequence[np.ndarray], widths: S
         x2 = x.reshape(b * sp, hidden)
         n_hi, n_lo, rstd_f, _ = kernels.rmsnorm_split(x2, final_norm, arch.rms_eps)
         t = b * s
-        real = n_hi.view(b, sp, hidden)[:, :s].reshape(t, hidden), \
-            n_lo.view(b, sp, hidden)[:, :s].reshape(t, hidden)
         vocab = head.shape[0]
-        logits = torch.empty((t, vocab), dtype=torch.float32, device=dev)
-        kernels.gemm(real[0], real[1], head, None, logits, m=t, n=vocab, k=hidden, a_kmajor=True,
-                     b_kmajor=True, lda=hidden, ldb=hidden, ldc=vocab, precision=2)
-        # d(mean CE)/dlogits = (softmax - onehot) / t, one row-wise kernel
-        g_hi, g_lo = kernels.ce_grad_split(logits, labels.reshape(-1).contiguous(), 1.0 / t)
+        logits = _head_logits((n_hi, n_lo), head, b, s)
+        if target is None:
+            # d(mean CE)/dlogits = (softmax - onehot) / t, one row-wise kernel
+            g_hi, g_lo = kernels.ce_grad_split(logits, labels.reshape(-1).contiguous(), 1.0 / t)
+        else:
+            weight = torch.full((t,), 1.0 / t, dtype=torch.float32, device=dev)
+            each, (g_hi, g_lo) = kernels.distill_topk_grad(
+                logits, *target, weight=weight, temperature=temperature, split=True)
+            loss += each.double().sum()
         del logits
         dh = torch.empty((t, hidden), dtype=torch.float32, device=dev)
         kernels.gemm(g_hi, g_lo, head, None, dh, m=t, n=hidden, k=vocab, a_kmajor=True,
@@ -206,13 +283,12 @@ def score_widths(model: SyntheticModel, batches: Sequence[np.ndarray], widths: S
 
     schedule = [(w, [w]) for w in widths] if gradient_source == "own_width" else [(widths[-1], widths)]
     done = 0
-    dist = dist or DistContext()
-    mine = list(batches)[dist.rank::dist.world]
+    losses = {bits: torch.zeros((), dtype=torch.float64, device=dev) for bits, _ in schedule}
     for anchor_bits, scored in schedule:
         set_anchors(anchor_bits)
         active["bits"] = scored
-        for batch in mine:
-            backward_pass(batch)
+        for batch, target in zip(mine, targets):
+            backward_pass(batch, target, losses[anchor_bits])
             done += 1
             if progress is not None:
                 progress(f"  scoring: backward {done}/{len(mine) * len(schedule)} "
@@ -222,10 +298,15 @@ def score_widths(model: SyntheticModel, batches: Sequence[np.ndarray], widths: S
         stacked = torch.stack([acc[p] for p in names])
         dist.all_reduce_(stacked)
         acc = {p: stacked[i] for i, p in enumerate(names)}
+        if distills:
+            for value in losses.values():
+                dist.all_reduce_(value)
     torch.cuda.synchronize(dev)
     for blk in blocks:
         for layer in blk.layers.values():
             layer.grad_ready.clear()
             layer.grad = None
     scores = {p: {w: float(acc[p][j].item()) for j, w in enumerate(widths)} for p in shapes}
-    return SensitivityScores(scores, shapes, tuple(skipped), time.perf_counter() - started)
+    mean = {bits: float(v.item()) / max(1, len(batches)) for bits, v in losses.items()}
+    return SensitivityScores(scores, shapes, tuple(skipped), time.perf_counter() - started,
+                             mean if distills else None)
