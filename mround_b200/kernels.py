@@ -8,9 +8,11 @@ runs only on the GPU: a CPU tensor is refused with ``PlatformError``.
 
 from __future__ import annotations
 
+from ctypes import addressof
+
 import torch
 
-from mround_b200._native import check, lib
+from mround_b200._native import LinearOperand, RotaryHeads, check, lib
 from mround_b200.exceptions import PlatformError, SchemeError
 
 __all__ = [
@@ -816,30 +818,37 @@ def _dtype_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _rotary(q, k, cos, sin, positions, layout, out, transposed):
-    from mround_b200._native import RotaryHeads
+def _rotary_heads(name: str, x, y, b: int, s: int, d: int, dtype) -> RotaryHeads:
+    """``mr_rotary_heads`` of the heads ``x``, turned into ``y`` (of x's shape)."""
+    bx, px, heads, dx = x.shape
+    if bx != b or px != s or dx != d or x.dtype != dtype or heads == 0:
+        raise SchemeError(f"{name} is {tuple(x.shape)} {x.dtype}, expected ({b}, {s}, at least one "
+                          f"head, {d}) {dtype}")
+    xb, xs, xh, xd = x.stride()
+    yb, ys, yh, yd = y.stride()
+    if (xd != 1 or yd != 1) and d > 1:
+        raise SchemeError(f"{name}'s last dimension must be contiguous")
+    return RotaryHeads(x.data_ptr(), y.data_ptr(), xb, xs, xh, yb, ys, yh, heads)
 
+
+def _rotary(q, k, cos, sin, positions, layout, out, transposed):
     inter = _interleaved(layout)
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise SchemeError("q and k are (batch, positions, heads, head dim)")
-    b, s, hq, d = q.shape
+    b, s, _, d = q.shape
+    dtype = q.dtype
     if out is None:
         out = (torch.empty_like(q), None if k is None else torch.empty_like(k))
+    else:
+        for x, y in ((q, out[0]), (k, out[1])):
+            if (x is None) != (y is None):
+                raise SchemeError("out is a (q, k) pair with k None exactly where k is")
+            if x is not None and (y.shape != x.shape or y.dtype != dtype):
+                raise SchemeError(f"an output is {tuple(y.shape)} {y.dtype}, expected "
+                                  f"{tuple(x.shape)} {dtype}")
     yq, yk = out
     dev = _device_of("q k cos sin positions out_q out_k", q, k, cos, sin, positions, yq, yk)
     code = _dtype_code(q, "q")
-    if (k is None) != (yk is None):
-        raise SchemeError("out is a (q, k) pair with k None exactly where k is")
-    for name, x, y in (("q", q, yq), ("k", k, yk)):
-        if x is None:
-            continue
-        if x.dtype != q.dtype or y.dtype != q.dtype:
-            raise SchemeError(f"{name} and its output must be {q.dtype}")
-        if x.shape[:2] != (b, s) or x.shape[3] != d or y.shape != x.shape:
-            raise SchemeError(f"{name} has shape {tuple(x.shape)} and output {tuple(y.shape)}, "
-                              f"expected ({b}, {s}, heads, {d})")
-        if (x.stride(3) != 1 or y.stride(3) != 1) and d > 1:
-            raise SchemeError(f"{name}'s last dimension must be contiguous")
     if cos.dim() != 2 or cos.shape != sin.shape:
         raise SchemeError(f"cos and sin are (positions, rotated columns / 2) tables, got "
                           f"{tuple(cos.shape)} and {tuple(sin.shape)}")
@@ -848,34 +857,26 @@ def _rotary(q, k, cos, sin, positions, layout, out, transposed):
         raise SchemeError(f"tables of {half} pairs do not fit head dim {d} (at most 1024)")
     pos_ptr, pos64, pos_stride = None, 0, 0
     if positions is not None:
-        if positions.dtype not in (torch.int64, torch.int32):
+        pos64 = positions.dtype == torch.int64
+        if not pos64 and positions.dtype != torch.int32:
             raise SchemeError(f"positions must be int64 or int32, got {positions.dtype}")
-        if positions.shape not in ((s,), (b, s)) or not positions.is_contiguous():
-            raise SchemeError(f"positions must be a contiguous ({s},) or ({b}, {s}) tensor")
-        pos_ptr, pos64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-        pos_stride = s if positions.dim() == 2 else 0
+        shape = tuple(positions.shape)
+        if shape == (b, s):
+            pos_stride = s
+        elif shape != (s,):
+            raise SchemeError(f"positions must be ({s},) or ({b}, {s}), got {shape}")
+        if not positions.is_contiguous():
+            raise SchemeError("positions must be contiguous")
+        pos_ptr = positions.data_ptr()
     elif s > rows:
         raise SchemeError(f"{s} positions but tables of {rows} rows")
-    if hq == 0 or (k is not None and k.shape[2] == 0):
-        raise SchemeError("q and k need at least one head")
-    if b * s == 0:
-        return out
-    heads = [None, None]
-    for i, (x, y) in enumerate(((q, yq), (k, yk))):
-        if x is not None:
-            sx, sy = x.stride(), y.stride()
-            heads[i] = RotaryHeads(x.data_ptr(), y.data_ptr(), sx[0], sx[1], sx[2], sy[0], sy[1],
-                                   sy[2], x.shape[2])
-    _launch("mr_rotary", dev, _ref(heads[0]), _ref(heads[1]), _ptr(cos, torch.float32, "cos"),
-            _ptr(sin, torch.float32, "sin"), rows, pos_ptr, pos64, pos_stride, b, s, d, 2 * half,
-            inter, transposed, code)
+    hq = _rotary_heads("q", q, yq, b, s, d, dtype)
+    hk = None if k is None else _rotary_heads("k", k, yk, b, s, d, dtype)
+    if b * s:
+        _launch("mr_rotary", dev, addressof(hq), None if hk is None else addressof(hk),
+                _ptr(cos, torch.float32, "cos"), _ptr(sin, torch.float32, "sin"), rows, pos_ptr,
+                pos64, pos_stride, b, s, d, 2 * half, inter, transposed, code)
     return out
-
-
-def _ref(struct):
-    import ctypes
-
-    return None if struct is None else ctypes.addressof(struct)
 
 
 def rotary(q, k, cos, sin, *, positions=None, layout: str = "half", out=None):
@@ -907,9 +908,11 @@ def _logit_rows(logits):
     if logits.dim() != 2:
         raise SchemeError(f"logits are (rows, vocabulary), got shape {tuple(logits.shape)}")
     rows, n = logits.shape
-    if n == 0 or (n > 1 and logits.stride(1) != 1) or n > 0x7FFFFFFF:
+    ld, inner = logits.stride()
+    if n == 0 or (n > 1 and inner != 1) or n > 0x7FFFFFFF:
         raise SchemeError("the logits' columns must be contiguous, at least one")
-    ld = logits.stride(0) if rows > 1 else n
+    if rows <= 1:
+        ld = n
     if ld < n:
         raise SchemeError("the logits' rows overlap")
     return rows, n, ld
@@ -927,8 +930,8 @@ def topk_logits(logits, k: int):
     code = _dtype_code(logits, "logits")
     if not 1 <= k <= min(n, MAX_TOPK):
         raise SchemeError(f"k must be 1 to {min(n, MAX_TOPK)}, got {k}")
-    values = torch.empty((rows, k), dtype=torch.float32, device=logits.device)
-    index = torch.empty((rows, k), dtype=torch.int64, device=logits.device)
+    values = logits.new_empty((rows, k), dtype=torch.float32)
+    index = logits.new_empty((rows, k), dtype=torch.int64)
     if rows:
         _launch("mr_topk_logits", dev, logits.data_ptr(), rows, n, ld, k, code, values.data_ptr(),
                 index.data_ptr())
@@ -939,10 +942,11 @@ def _distill(logits, t_logits, t_index, temperature, weight, loss, grad, pair, l
     dev = _device_of("logits t_logits t_index weight out", logits, t_logits, t_index, weight, grad)
     rows, n, ld = _logit_rows(logits)
     code = _dtype_code(logits, "logits")
-    if t_logits.dim() != 2 or t_logits.shape != t_index.shape or t_logits.shape[0] != rows:
-        raise SchemeError(f"t_logits and t_index are ({rows}, k), got {tuple(t_logits.shape)} and "
+    shape = tuple(t_logits.shape)
+    if len(shape) != 2 or shape[0] != rows or tuple(t_index.shape) != shape:
+        raise SchemeError(f"t_logits and t_index are ({rows}, k), got {shape} and "
                           f"{tuple(t_index.shape)}")
-    k = t_logits.shape[1]
+    k = shape[1]
     if not 1 <= k <= MAX_TOPK:
         raise SchemeError(f"1 to {MAX_TOPK} teacher logits per row, got {k}")
     if not 1e-3 <= float(temperature) <= 1e3:
@@ -968,7 +972,7 @@ def distill_topk(logits, t_logits, t_index, *, temperature: float = 1.0, weight=
     occurs, one beyond the vocabulary makes its row NaN.  ``weight``: float32
     (rows,); a row of weight 0, or without an entry, gives 0 whatever it holds.
     Returns float32 (rows,)."""
-    loss = torch.empty(logits.shape[:1], dtype=torch.float32, device=logits.device)
+    loss = logits.new_empty(len(logits), dtype=torch.float32)
     _distill(logits, t_logits, t_index, temperature, weight, loss, None, (None, None), 0)
     return loss
 
@@ -982,7 +986,7 @@ def distill_topk_grad(logits, t_logits, t_index, *, temperature: float = 1.0, we
     The gradient has the logits' type, in ``out`` when given (contiguous
     columns; ``logits`` itself may be given), or with ``split`` is the bf16
     (hi, lo) pair that :func:`gemm` takes.  Returns (loss, gradient)."""
-    loss = torch.empty(logits.shape[:1], dtype=torch.float32, device=logits.device)
+    loss = logits.new_empty(len(logits), dtype=torch.float32)
     if split:
         if out is not None:
             raise SchemeError("a split gradient is allocated by the call")
@@ -991,10 +995,12 @@ def distill_topk_grad(logits, t_logits, t_index, *, temperature: float = 1.0, we
                  logits.shape[-1])
         return loss, pair
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    elif out.shape != logits.shape or out.dtype != logits.dtype:
-        raise SchemeError(f"out must be {tuple(logits.shape)} {logits.dtype}")
-    _, _, ldg = _logit_rows(out)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        ldg = logits.shape[-1]
+    else:
+        if out.shape != logits.shape or out.dtype != logits.dtype:
+            raise SchemeError(f"out must be {tuple(logits.shape)} {logits.dtype}")
+        _, _, ldg = _logit_rows(out)
     _distill(logits, t_logits, t_index, temperature, weight, loss, out, (None, None), ldg)
     return loss, out
 
@@ -1012,36 +1018,38 @@ def _act_code(act: str) -> int:
 
 def _parts(t, name: str):
     """(hi, lo or None) of a bf16 operand given as a tensor or as a pair."""
-    hi, lo = t if isinstance(t, (tuple, list)) else (t, None)
-    for part in (hi, lo):
-        if part is None and part is lo:
-            continue
-        if part.dim() != 2 or part.dtype != torch.bfloat16:
-            raise SchemeError(f"{name} must be a 2-D bfloat16 tensor or a (hi, lo) pair of them")
-        if part.shape != hi.shape or part.stride() != hi.stride():
+    if isinstance(t, torch.Tensor):
+        if t.dim() == 2 and t.dtype == torch.bfloat16:
+            return t, None
+    elif len(t) == 2 and all(p.dim() == 2 and p.dtype == torch.bfloat16 for p in t):
+        hi, lo = t
+        if lo.shape != hi.shape or lo.stride() != hi.stride():
             raise SchemeError(f"{name}'s parts must have one shape and layout")
-    return hi, lo
+        return hi, lo
+    raise SchemeError(f"{name} must be a 2-D bfloat16 tensor or a (hi, lo) pair of them")
 
 
 def _operand(parts, name: str, kmajor: bool):
     """``mr_linear_operand`` of parts whose columns (K-major) or rows are k."""
-    from mround_b200._native import LinearOperand
-
     hi, lo = parts
     rows, cols = hi.shape
-    ld = hi.stride(0) if rows > 1 else -(-cols // 8) * 8
-    if (cols > 1 and hi.stride(1) != 1) or ld < cols or ld % 8:
+    ld, inner = hi.stride()
+    if rows == 1:
+        ld = -(-cols // 8) * 8
+    if (inner != 1 and cols > 1) or ld < cols or ld % 8:
         raise SchemeError(f"{name} needs contiguous columns and a row stride that is a multiple "
                           f"of 8, got strides {hi.stride()}")
-    return LinearOperand(hi.data_ptr(), None if lo is None else lo.data_ptr(), ld, int(kmajor))
+    return LinearOperand(hi.data_ptr(), None if lo is None else lo.data_ptr(), ld, kmajor)
 
 
 def _row_stride(t, rows: int, cols: int, dtypes, name: str) -> int:
-    if t.dtype not in dtypes or t.shape != (rows, cols):
+    ld, inner = t.stride() if t.dim() == 2 else (0, 0)
+    if t.dtype not in dtypes or tuple(t.shape) != (rows, cols):
         raise SchemeError(f"{name} must be ({rows}, {cols}) of {dtypes}, got {tuple(t.shape)} "
                           f"{t.dtype}")
-    ld = t.stride(0) if rows > 1 else cols
-    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+    if rows == 1:
+        ld = cols
+    if (inner != 1 and cols > 1) or ld < cols:
         raise SchemeError(f"{name} needs contiguous columns in rows that do not overlap")
     return ld
 
@@ -1055,10 +1063,13 @@ def _linear_call(dev, x, w, toks, feats, k, act, bias, residual, ldr, out, lo, t
     if timing:
         start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         start.record()
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    _launch("mr_linear", dev, _ref(x), _ref(w), toks, feats, k, act, ptr(bias), ptr(residual),
+    _launch("mr_linear", dev, addressof(x), addressof(w), toks, feats, k, act,
+            None if bias is None else bias.data_ptr(),
+            None if residual is None else residual.data_ptr(),
             0 if residual is None else DTYPES[residual.dtype], ldr, out.data_ptr(),
-            DTYPES[out.dtype], ptr(lo), ptr(t32), ldo, ptr(pre), ldp, splits)
+            DTYPES[out.dtype], None if lo is None else lo.data_ptr(),
+            None if t32 is None else t32.data_ptr(), ldo, None if pre is None else pre.data_ptr(),
+            ldp, splits)
     if timing:
         end.record()
         products = 1 + (x.lo is not None) + (w.lo is not None)
@@ -1101,17 +1112,20 @@ def linear(x, w, *, bias=None, act: str = "none", residual=None, out=None, dtype
     if splits is not None and splits not in LINEAR_SPLITS:
         raise SchemeError(f"splits must be one of {LINEAR_SPLITS}, got {splits}")
     feats = rows // 2 if act == "swiglu" else rows
-    lo = None
+    lo, ldo = None, feats
     if split:
         if out is not None or dtype is not None:
             raise SchemeError("a split output is allocated by the call")
         out, lo = _pair((toks, feats), xp[0].device)
     elif out is None:
-        out = torch.empty((toks, feats), device=xp[0].device,
-                          dtype=dtype or (torch.bfloat16 if xp[1] is None else torch.float32))
-    elif dtype is not None and out.dtype != dtype:
-        raise SchemeError(f"out is {out.dtype}, not {dtype}")
-    ldo = _row_stride(out, toks, feats, _LINEAR_OUT, "out")
+        dtype = dtype or (torch.bfloat16 if xp[1] is None else torch.float32)
+        if dtype not in _LINEAR_OUT:
+            raise SchemeError(f"dtype must be float32 or bfloat16, got {dtype}")
+        out = xp[0].new_empty((toks, feats), dtype=dtype)
+    else:
+        if dtype is not None and out.dtype != dtype:
+            raise SchemeError(f"out is {out.dtype}, not {dtype}")
+        ldo = _row_stride(out, toks, feats, _LINEAR_OUT, "out")
     if t32 is not None:
         if _row_stride(t32, toks, feats, (torch.float32,), "t32") != ldo:
             raise SchemeError("t32 must have the output's row stride")
