@@ -9,16 +9,17 @@
 // is the inverse only where c^2 + s^2 = 1: tables may carry a factor (YaRN's
 // attention scaling), which the gradient carries too.
 //
-// HBM-bound: each value is read and written once.  A thread keeps one unit of
-// columns (16 bytes of each half, or 16 bytes of interleaved pairs), reads its
-// cosines and sines once and walks the token's heads four at a time, so that
-// four heads' loads are in flight and the tables cost one read per four heads.
-// A launch takes query and key heads together: at one token the launch itself
-// is the cost.
+// HBM-bound: each value is read and written once (16384 tokens x 32 heads of 128
+// float32: 92 us, 5.8 TB/s).  A thread keeps one unit of columns (two vectors:
+// 16 bytes of each half, or 32 bytes of interleaved pairs), reads its cosines
+// and sines once and walks the token's heads four at a time, so that four heads'
+// loads are in flight and the tables cost one read per four heads.  A block
+// takes as many tokens as fill 128 threads.  A launch takes query and key heads
+// together: at one token the launch itself is the cost.
 //
 // Tensors whose addresses or strides do not divide into 16 bytes, or whose
-// halves do not divide into whole vectors, take the one-column form of the
-// same kernel.
+// halves do not divide into whole vectors, take narrower forms of the same
+// kernel: vectors of two columns, or one column at a time.
 
 #include <type_traits>
 
@@ -26,6 +27,47 @@
 
 namespace mr {
 namespace {
+
+// Two values.
+template <typename T>
+struct Pair {
+  typename std::conditional<sizeof(T) == 4, uint2, uint32_t>::type raw;
+  __device__ __forceinline__ void get(float (&f)[2]) const {
+    if constexpr (sizeof(T) == 4) {
+      f[0] = __uint_as_float(raw.x);
+      f[1] = __uint_as_float(raw.y);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&raw));
+      f[0] = p.x;
+      f[1] = p.y;
+    } else {
+      f[0] = __uint_as_float(raw << 16);
+      f[1] = __uint_as_float(raw & 0xFFFF0000u);
+    }
+  }
+  __device__ __forceinline__ void put(const float (&f)[2]) {
+    if constexpr (sizeof(T) == 4) {
+      raw = make_uint2(__float_as_uint(f[0]), __float_as_uint(f[1]));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 p = __floats2half2_rn(f[0], f[1]);
+      raw = *reinterpret_cast<const uint32_t*>(&p);
+    } else {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(f[0], f[1]);
+      raw = *reinterpret_cast<const uint32_t*>(&p);
+    }
+  }
+};
+
+template <typename T>
+struct One {
+  T raw;
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f32(raw); }
+  __device__ __forceinline__ void put(const float (&f)[1]) { raw = from_f32<T>(f[0]); }
+};
+
+template <typename T, int V>
+using VecOf = typename std::conditional<
+    V == 1, One<T>, typename std::conditional<V == 2, Pair<T>, Vec16<T>>::type>::type;
 
 struct RotaryHeads {
   const void* x;
@@ -55,32 +97,33 @@ __device__ __forceinline__ int64_t position_of(const RotaryArgs& a, int64_t b, i
                  : int64_t(static_cast<const int32_t*>(a.positions)[i]);
 }
 
-// blockDim.x: column units of a head (rotated units first, then copied ones);
-// blockDim.y: head lanes; at most 256 threads, or 1024 one-column units.
-// V columns per vector: 16 bytes, or 1.
+// blockDim.x: column units of a head (rotated units of two vectors first, then
+// copied ones of one); blockDim.y: head lanes; blockDim.z: tokens.  V columns
+// per vector: 16 bytes, two columns, or one.
 template <typename T, bool kInterleaved, bool kTransposed, int V>
-__global__ void __launch_bounds__(V > 1 ? 256 : 1024) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr int kPairs = kInterleaved && V > 1 ? V / 2 : V;  // pairs of one rotated unit
-  const int turned = a.r / (2 * kPairs);                     // rotated units per head
+__global__ void __launch_bounds__(V * sizeof(T) == 16 ? 256 : V > 1 ? 512 : 1024)
+    rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  using Vec = VecOf<T, V>;
+  using Raw = decltype(Vec::raw);
+  const int turned = a.r / (2 * V);  // rotated units per head, V pairs each
   const int u = threadIdx.x;
   const int heads = a.q.heads + a.k.heads;
   const bool rotates = u < turned;
-  // first column of the unit's (first) vector, and of its second one
-  const int c0 = !rotates ? a.r + (u - turned) * V
-                          : (kInterleaved ? u * 2 * kPairs : u * kPairs);
-  const int c1 = kInterleaved ? c0 + 1 : c0 + a.r / 2;  // whole interleaved vectors hold both
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+  const int c0 = !rotates ? a.r + (u - turned) * V : kInterleaved ? u * 2 * V : u * V;
+  const int c1 = kInterleaved ? c0 + V : c0 + a.r / 2;
+  const int64_t step = int64_t(gridDim.x) * blockDim.z;
+  for (int64_t t = int64_t(blockIdx.x) * blockDim.z + threadIdx.z; t < a.tokens; t += step) {
     const int64_t b = t / a.seq;
     const int s = int(t - b * a.seq);
-    float cs[kPairs], sn[kPairs];
+    float cs[V], sn[V];
     if (rotates) {
       const int64_t p = position_of(a, b, s);
       if (p >= 0 && p < a.table_rows) {
-        const float* cr = a.cosv + p * (a.r / 2) + u * kPairs;
-        const float* sr = a.sinv + p * (a.r / 2) + u * kPairs;
-        if constexpr (kPairs % 4 == 0) {
+        const float* cr = a.cosv + p * (a.r / 2) + u * V;
+        const float* sr = a.sinv + p * (a.r / 2) + u * V;
+        if constexpr (V % 4 == 0) {
 #pragma unroll
-          for (int i = 0; i < kPairs; i += 4) {
+          for (int i = 0; i < V; i += 4) {
             const float4 c4 = *reinterpret_cast<const float4*>(cr + i);
             const float4 s4 = *reinterpret_cast<const float4*>(sr + i);
             cs[i] = c4.x; cs[i + 1] = c4.y; cs[i + 2] = c4.z; cs[i + 3] = c4.w;
@@ -88,120 +131,105 @@ __global__ void __launch_bounds__(V > 1 ? 256 : 1024) rotary_kernel(const __grid
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < kPairs; ++i) {
+          for (int i = 0; i < V; ++i) {
             cs[i] = cr[i];
             sn[i] = sr[i];
           }
         }
       } else {  // outside the tables: no angle to turn by
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) cs[i] = sn[i] = __int_as_float(0x7fffffff);
+        for (int i = 0; i < V; ++i) cs[i] = sn[i] = __int_as_float(0x7fffffff);
       }
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i)
+      for (int i = 0; i < V; ++i)
         if (kTransposed) sn[i] = -sn[i];
     }
     for (int h0 = threadIdx.y; h0 < heads; h0 += blockDim.y * kHeadsAtOnce) {
       const T* src[kHeadsAtOnce];
       T* dst[kHeadsAtOnce];
+      Vec v0[kHeadsAtOnce], v1[kHeadsAtOnce];
 #pragma unroll
       for (int i = 0; i < kHeadsAtOnce; ++i) {
         int h = h0 + i * blockDim.y;
-        if (h >= heads) {
-          src[i] = nullptr;
-          continue;
-        }
+        src[i] = nullptr;
+        if (h >= heads) continue;
         const RotaryHeads& w = h < a.q.heads ? a.q : a.k;
         if (h >= a.q.heads) h -= a.q.heads;
         src[i] = static_cast<const T*>(w.x) + b * w.xb + s * w.xs + h * w.xh;
         dst[i] = static_cast<T*>(w.y) + b * w.yb + s * w.ys + h * w.yh;
+        v0[i].raw = *reinterpret_cast<const Raw*>(src[i] + c0);
+        if (rotates) v1[i].raw = *reinterpret_cast<const Raw*>(src[i] + c1);
       }
-      if constexpr (V > 1) {
-        Vec16<T> v0[kHeadsAtOnce], v1[kHeadsAtOnce];
 #pragma unroll
-        for (int i = 0; i < kHeadsAtOnce; ++i) {
-          if (!src[i]) continue;
-          v0[i].raw = *reinterpret_cast<const uint4*>(src[i] + c0);
-          if (!kInterleaved && rotates) v1[i].raw = *reinterpret_cast<const uint4*>(src[i] + c1);
-        }
+      for (int i = 0; i < kHeadsAtOnce; ++i) {
+        if (!src[i]) continue;
+        if (rotates) {
+          float f0[V], f1[V];
+          v0[i].get(f0);
+          v1[i].get(f1);
+          if constexpr (kInterleaved && V > 1) {  // pairs of neighbours in each vector
 #pragma unroll
-        for (int i = 0; i < kHeadsAtOnce; ++i) {
-          if (!src[i]) continue;
-          if (rotates) {
-            float f0[V];
-            v0[i].get(f0);
-            if constexpr (kInterleaved) {
-#pragma unroll
-              for (int j = 0; j < kPairs; ++j) {
-                const float x1 = f0[2 * j], x2 = f0[2 * j + 1];
-                f0[2 * j] = x1 * cs[j] - x2 * sn[j];
-                f0[2 * j + 1] = x1 * sn[j] + x2 * cs[j];
-              }
-            } else {
-              float f1[V];
-              v1[i].get(f1);
-#pragma unroll
-              for (int j = 0; j < V; ++j) {
-                const float x1 = f0[j], x2 = f1[j];
-                f0[j] = x1 * cs[j] - x2 * sn[j];
-                f1[j] = x1 * sn[j] + x2 * cs[j];
-              }
-              v1[i].put(f1);
-              *reinterpret_cast<uint4*>(dst[i] + c1) = v1[i].raw;
+            for (int j = 0; j < V / 2; ++j) {
+              const float x1 = f0[2 * j], x2 = f0[2 * j + 1];
+              f0[2 * j] = x1 * cs[j] - x2 * sn[j];
+              f0[2 * j + 1] = x1 * sn[j] + x2 * cs[j];
+              const float x3 = f1[2 * j], x4 = f1[2 * j + 1];
+              f1[2 * j] = x3 * cs[V / 2 + j] - x4 * sn[V / 2 + j];
+              f1[2 * j + 1] = x3 * sn[V / 2 + j] + x4 * cs[V / 2 + j];
             }
-            v0[i].put(f0);
-          }
-          *reinterpret_cast<uint4*>(dst[i] + c0) = v0[i].raw;
-        }
-      } else {
-        T e0[kHeadsAtOnce], e1[kHeadsAtOnce];
-#pragma unroll
-        for (int i = 0; i < kHeadsAtOnce; ++i) {
-          if (!src[i]) continue;
-          e0[i] = src[i][c0];
-          if (rotates) e1[i] = src[i][c1];
-        }
-#pragma unroll
-        for (int i = 0; i < kHeadsAtOnce; ++i) {
-          if (!src[i]) continue;
-          if (rotates) {
-            const float x1 = to_f32(e0[i]), x2 = to_f32(e1[i]);
-            dst[i][c0] = from_f32<T>(x1 * cs[0] - x2 * sn[0]);
-            dst[i][c1] = from_f32<T>(x1 * sn[0] + x2 * cs[0]);
           } else {
-            dst[i][c0] = e0[i];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const float x1 = f0[j], x2 = f1[j];
+              f0[j] = x1 * cs[j] - x2 * sn[j];
+              f1[j] = x1 * sn[j] + x2 * cs[j];
+            }
           }
+          v0[i].put(f0);
+          v1[i].put(f1);
+          *reinterpret_cast<Raw*>(dst[i] + c1) = v1[i].raw;
         }
+        *reinterpret_cast<Raw*>(dst[i] + c0) = v0[i].raw;
       }
     }
   }
 }
 
-bool heads_aligned(const RotaryHeads& h, int v) {
-  return !h.heads || (aligned16(h.x) && aligned16(h.y) && h.xb % v == 0 && h.xs % v == 0 &&
-                      h.xh % v == 0 && h.yb % v == 0 && h.ys % v == 0 && h.yh % v == 0);
+// Whether addresses and strides divide into vectors of v columns.
+bool heads_divide(const RotaryHeads& h, int v, int elt) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(h.x) | reinterpret_cast<uintptr_t>(h.y);
+  return !h.heads || (at % (v * elt) == 0 && h.xb % v == 0 && h.xs % v == 0 && h.xh % v == 0 &&
+                      h.yb % v == 0 && h.ys % v == 0 && h.yh % v == 0);
+}
+
+template <typename T, bool kInterleaved, bool kTransposed, int V>
+int launch_rotary_as(const RotaryArgs& a, cudaStream_t stream) {
+  const int heads = a.q.heads + a.k.heads;
+  const int units = a.r / (2 * V) + (a.d - a.r) / V;
+  int lanes = (heads + kHeadsAtOnce - 1) / kHeadsAtOnce;
+  const int most = 256 / units > 0 ? 256 / units : 1;
+  if (lanes > most) lanes = most;
+  int z = 128 / (units * lanes);  // blockDim.z is at most 64
+  z = z < 1 ? 1 : z > 64 ? 64 : z;
+  if (z > a.tokens) z = int(a.tokens);
+  const int64_t blocks = (a.tokens + z - 1) / z;
+  const unsigned grid = unsigned(blocks < 0x7fffffff ? blocks : 0x7fffffff);
+  rotary_kernel<T, kInterleaved, kTransposed, V><<<grid, dim3(units, lanes, z), 0, stream>>>(a);
+  return launch_status();
 }
 
 template <typename T, bool kInterleaved, bool kTransposed>
 int launch_rotary(const RotaryArgs& a, cudaStream_t stream) {
-  constexpr int kV = 16 / int(sizeof(T));
-  const int heads = a.q.heads + a.k.heads;
-  // whole vectors: of each half, or of pairs; the copied columns; the tables
-  const bool wide = (kInterleaved ? a.r % kV == 0 : (a.r / 2) % kV == 0) && a.d % kV == 0 &&
-                    heads_aligned(a.q, kV) && heads_aligned(a.k, kV) && aligned16(a.cosv) &&
-                    aligned16(a.sinv);
-  const int pairs = !wide ? 1 : kInterleaved ? kV / 2 : kV;
-  const int units = a.r / (2 * pairs) + (a.d - a.r) / (wide ? kV : 1);
-  int lanes = (heads + kHeadsAtOnce - 1) / kHeadsAtOnce;
-  const int most = 256 / units > 0 ? 256 / units : 1;
-  if (lanes > most) lanes = most;
-  const unsigned grid = unsigned(a.tokens < 0x7fffffff ? a.tokens : 0x7fffffff);
-  const dim3 block(units, lanes);
-  if (wide)
-    rotary_kernel<T, kInterleaved, kTransposed, kV><<<grid, block, 0, stream>>>(a);
-  else
-    rotary_kernel<T, kInterleaved, kTransposed, 1><<<grid, block, 0, stream>>>(a);
-  return launch_status();
+  constexpr int kElt = int(sizeof(T)), kWide = 16 / kElt;
+  // whole units of two vectors of v columns, and whole vectors of copied ones
+  auto divides = [&](int v) {
+    return a.r % (2 * v) == 0 && a.d % v == 0 && heads_divide(a.q, v, kElt) &&
+           heads_divide(a.k, v, kElt);
+  };
+  if (divides(kWide) && aligned16(a.cosv) && aligned16(a.sinv))
+    return launch_rotary_as<T, kInterleaved, kTransposed, kWide>(a, stream);
+  if (divides(2)) return launch_rotary_as<T, kInterleaved, kTransposed, 2>(a, stream);
+  return launch_rotary_as<T, kInterleaved, kTransposed, 1>(a, stream);
 }
 
 // Operand forms for the decoder block (float32 rows of [q | k | v] heads in,

@@ -63,6 +63,9 @@ CASES = [
     (2, 5, 2, 1, 7, 6),
     (1, 3, 40, 8, 256, 192),
     (1, 2, 2, 2, 1024, 1024),
+    (2, 9, 3, 2, 36, 20),
+    (1, 5, 7, 1, 106, 16),
+    (1, 2, 1, 1, 1022, 500),
 ]
 
 
