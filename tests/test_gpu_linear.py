@@ -5,7 +5,8 @@ rounding (or truncation) of at most 2**-23 of a partial sum per 16 k and
 product, and per CTA that shares k; with S = sum |x||w| every partial sum is at
 most S, so z is within dz = (products * (k / 16 + 1) + 16) * 2**-23 * S (16
 covers the join, the bias and 8 shares).  Activations have slopes of at most
-1.13 and are evaluated to 2**-20 of |z|.  bf16 rounds by at most 2**-8 of the
+1.13 and are evaluated to 2**-20 of |z| (where bf16 alone is written, to 2**-13
+of the value: test_activation_over_its_range).  bf16 rounds by at most 2**-8 of the
 value, a hi/lo pair leaves 2**-16, tf32 2**-11, float32 2**-24.
 """
 
@@ -369,3 +370,38 @@ def test_refusals_on_the_device(K):
         K.linear_bwd(z(4, 15), x, w)
     with pytest.raises(PlatformError):
         K.linear(x, w.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "swiglu"])
+def test_activation_over_its_range(K, act, dtype):
+    """Each activation alone (one column, weight 1) from far below to far above
+    zero, where the tails lose their size first.
+
+    bf16 results hold their own size: half a step, 2^-8 of the value, and the
+    activation's 2^-13, down to 2^-100 (smaller ones may be zero).  float32 ones
+    hold the size of z: each form is z times a factor of at most 1 that a few
+    rounded steps compute, less than 2^-20 with what the exponent's argument,
+    at most 128 where the factor is above 2^-126, has lost (2^-24 of it)."""
+    z = torch.linspace(-14, 14, 4093, device="cuda").to(torch.bfloat16)
+    w = torch.zeros(16 if act == "swiglu" else 8, 8, dtype=torch.bfloat16, device="cuda")
+    w[:, 0] = 1
+    x = torch.zeros(z.numel(), 8, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = z
+    if act == "swiglu":  # silu(z) times 1
+        w[8:, 0], w[8:, 1], x[:, 1] = 0, 1, 1
+    out = K.linear(x, w, act=act, dtype=dtype).double()
+    d = z.double()
+    if act == "gelu":
+        want = 0.5 * d * torch.special.erfc(-d / math.sqrt(2))
+    elif act == "gelu_tanh":
+        want = d * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (d + 0.044715 * d ** 3))
+    else:
+        want = d * torch.sigmoid(d)
+    err = (out - want[:, None]).abs()
+    if dtype == torch.bfloat16:
+        bound = want.abs() * (2.0 ** -8 + 2.0 ** -13) + 2.0 ** -100
+    else:
+        bound = d.abs() * (2.0 ** -20 + 128 * 2.0 ** -24)
+    assert (err <= bound[:, None]).all()
