@@ -1148,7 +1148,8 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     ``dx = dz @ w`` and ``dw = dz.T @ x``, ``dz = dy * act'(pre)``, are ``dtype``
     (float32 or bfloat16; by default as the output of :func:`linear`), the bias
     gradient float32.  ``dz`` is carried as a bf16 pair into float32 gradients,
-    and rounded to bf16 once, like them, into bfloat16 ones."""
+    and rounded to bf16 once, like them, into bfloat16 ones; a bfloat16 ``dy``
+    without an activation is taken as it is."""
     code = _act_code(act)
     xp, wp = _parts(x, "x"), _parts(w, "w")
     dev = _device_of("dy x x_lo w w_lo pre", dy, *xp, *wp, pre)
@@ -1177,24 +1178,29 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
         if db is not None:
             db.zero_()
         return dx, dw, db
-    ldz = -(-rows // 8) * 8
-    hi = torch.empty((toks, ldz), dtype=torch.bfloat16, device=on)
-    # bf16 gradients: dz rounded as they are; the pair would double both products.
-    # A pair of operands keeps the float32-faithful form
-    lo = None
-    if out_dtype == torch.float32 or xp[1] is not None:
-        lo = torch.empty_like(hi)
+    # without an activation a bf16 dy is dz
+    as_is = (act == "none" and dy.dtype == torch.bfloat16 and xp[1] is None and
+             (toks == 1 or ldy % 8 == 0) and dy.data_ptr() % 16 == 0)
+    hi, lo, ldz = None, None, 0
+    if not as_is:
+        ldz = -(-rows // 8) * 8
+        hi = torch.empty((toks, ldz), dtype=torch.bfloat16, device=on)
+        # bf16 gradients: dz rounded as they are; the pair would double both
+        # products.  A pair of operands keeps the float32-faithful form
+        if out_dtype == torch.float32 or xp[1] is not None:
+            lo = torch.empty_like(hi)
     scratch = None
     if bias_grad:
         nbytes = int(lib().mr_act_grad_workspace_bytes(toks, feats, code))
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=on)
-    z = None if act == "none" else pre.data_ptr()
-    _launch("mr_act_grad", dev, dy.data_ptr(), DTYPES[dy.dtype], ldy, z, ldp, toks, feats, code,
-            hi.data_ptr(), None if lo is None else lo.data_ptr(), ldz,
-            None if db is None else db.data_ptr(),
-            None if scratch is None else scratch.data_ptr())
+    if bias_grad or not as_is:
+        z = None if act == "none" else pre.data_ptr()
+        _launch("mr_act_grad", dev, dy.data_ptr(), DTYPES[dy.dtype], ldy, z, ldp, toks, feats, code,
+                None if hi is None else hi.data_ptr(), None if lo is None else lo.data_ptr(), ldz,
+                None if db is None else db.data_ptr(),
+                None if scratch is None else scratch.data_ptr())
     n = splits or 0
-    dz = (hi[:, :rows], None if lo is None else lo[:, :rows])
+    dz = (dy, None) if as_is else (hi[:, :rows], None if lo is None else lo[:, :rows])
     _linear_call(dev, _operand(dz, "dz", True), w_op, toks, k, rows, 0, None, None, 0, dx, None,
                  None, k, None, 0, n)
     _linear_call(dev, _operand(dz, "dz", False), x_op, rows, k, toks, 0, None, None, 0, dw, None,

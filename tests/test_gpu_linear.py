@@ -405,3 +405,27 @@ def test_activation_over_its_range(K, act, dtype):
     else:
         bound = d.abs() * (2.0 ** -20 + 128 * 2.0 ** -24)
     assert (err <= bound[:, None]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,F,k", [(1, 8, 8), (1, 13, 40), (5, 24, 72), (129, 520, 136), (66, 33, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients_of_a_plain_linear(K, T, F, k, dtype):
+    """A bf16 dy without an activation, which is itself the products' operand
+    where its rows allow; a column slice of a wider one, whose neighbours must
+    not be read as its own; and one at an odd offset, which takes the copy."""
+    x, w, g = make(T, F, k, "none", 1, 5)
+    wide = torch.full((T, F + 24), math.nan, device="cuda", dtype=torch.bfloat16)
+    for first in (0, 8, 3):
+        dy = wide[:, first:first + F]
+        dy.copy_(torch.randn(T, F, device="cuda", generator=g))
+        dx, dw, db = K.linear_bwd(dy, x, w, bias_grad=True, dtype=dtype)
+        dx1, dw1, none = K.linear_bwd(dy, x, w, dtype=dtype)
+        assert none is None and torch.equal(dx, dx1) and torch.equal(dw, dw1)
+        for got, a, b in ((dx, dy.double(), w.double()), (dw, dy.double().t(), x.double())):
+            mass = a.abs() @ b.abs()
+            off = (2 * (a.shape[1] / 16 + 1) + 16) * 2.0 ** -23 * mass
+            close(got, a @ b, off, STEP[dtype])
+        off = (T / 4 + 8) * 2.0 ** -24 * dy.double().abs().sum(0)
+        close(db, dy.double().sum(0), off, 2.0 ** -24)
+        wide.fill_(math.nan)
