@@ -153,18 +153,8 @@ __device__ __forceinline__ float silu_rough(float g) {
   return __fdividef(g, 1.f + __expf(-g));
 }
 
-// z Phi(z).  Phi(-|z|) = t 2^(p(t) - z^2 log2(e) / 2) with t = 1 / (1 + |z| / 2)
-// and p the quartic of least largest error (fitted here for |z| <= 13.2, where
-// the tail leaves float32's range): relative error 5.5e-5.
 __device__ __forceinline__ float gelu_rough(float z) {
-  const float t = __fdividef(1.f, fmaf(0.5f, fabsf(z), 1.f));
-  float p = fmaf(0.375025481f, t, -1.147340059f);
-  p = fmaf(p, t, 0.711058915f);
-  p = fmaf(p, t, 1.383448601f);
-  p = fmaf(p, t, -2.322162628f);
-  float power;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(power) : "f"(fmaf(-0.72134752f * z, z, p)));
-  const float tail = t * power;
+  const float tail = gelu_tail(z);
   return z * (z < 0.f ? tail : 1.f - tail);
 }
 
