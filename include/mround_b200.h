@@ -671,8 +671,8 @@ int mr_linear(const mr_linear_operand* x, const mr_linear_operand* w, int64_t to
  * products mr_linear forms from it (dx = dz w, dw = dz^T x), and bias_grad = sum
  * over tokens of dz (float32).  bias_grad or hi (with lo) may be NULL.  dy
  * MR_F32 or MR_BF16, z the `pre` of mr_linear (NULL where act is none).  The
- * bias gradient needs a workspace of mr_act_grad_workspace_bytes, which must not
- * be shared by calls that may overlap.  At most 65535 * 64 tokens.
+ * bias gradient needs a workspace of mr_act_grad_workspace_bytes (0: none), which must
+ * not be shared by calls that may overlap.  At most 65535 * 64 tokens.
  */
 size_t mr_act_grad_workspace_bytes(int64_t toks, int64_t feats, int act);
 int mr_act_grad(const void* dy, int dy_dtype, int64_t ldy, const float* z, int64_t ldz,

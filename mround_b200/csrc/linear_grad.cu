@@ -206,7 +206,7 @@ int launch_act_grad(const void* dy, int64_t ldy, const float* z, int64_t ldz, in
 using namespace mr;
 
 extern "C" size_t mr_act_grad_workspace_bytes(int64_t toks, int64_t feats, int act) {
-  if (toks <= 0 || feats <= 0) return 0;
+  if (toks <= kGradTokens || feats <= 0) return 0;  // one strip is the sum itself
   return size_t(strips_of(toks)) * size_t(feats) * (act == MR_ACT_SWIGLU ? 2 : 1) * sizeof(float);
 }
 
@@ -219,9 +219,10 @@ extern "C" int mr_act_grad(const void* dy, int dy_dtype, int64_t ldy, const floa
       (hi && ldo < rows * feats) || (dy_dtype != MR_F32 && dy_dtype != MR_BF16) ||
       strips_of(toks) > 65535)
     return MR_ERR_ARGUMENT;
-  if (bias_grad && !workspace) return MR_ERR_WORKSPACE;
+  const bool one_strip = toks <= kGradTokens;
+  if (bias_grad && !workspace && !one_strip) return MR_ERR_WORKSPACE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float* sums = bias_grad ? static_cast<float*>(workspace) : nullptr;
+  float* sums = !bias_grad ? nullptr : one_strip ? bias_grad : static_cast<float*>(workspace);
   const bool wide = feats % 4 == 0 && ldy % 4 == 0 && (!z || ldz % 4 == 0) && (!hi || ldo % 4 == 0) &&
                     aligned16(z) &&
                     ((reinterpret_cast<uintptr_t>(hi) | reinterpret_cast<uintptr_t>(lo)) & 7u) == 0 &&
@@ -236,7 +237,7 @@ extern "C" int mr_act_grad(const void* dy, int dy_dtype, int64_t ldy, const floa
                                                       sums, st)
                   : launch_act_grad<__nv_bfloat16, 1>(dy, ldy, z, ldz, toks, n, act, hi, lo, ldo,
                                                       sums, st);
-  if (status != MR_OK || !bias_grad) return status;
+  if (status != MR_OK || !bias_grad || one_strip) return status;
   add_strips_kernel<<<unsigned((rows * feats + 255) / 256), 256, 0, st>>>(
       sums, int(strips_of(toks)), int(rows * feats), bias_grad);
   return launch_status();

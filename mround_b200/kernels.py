@@ -1153,7 +1153,7 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     code = _act_code(act)
     xp, wp = _parts(x, "x"), _parts(w, "w")
     dev = _device_of("dy x x_lo w w_lo pre", dy, *xp, *wp, pre)
-    on = dy.device
+    empty = dy.new_empty
     toks, k = xp[0].shape
     rows = wp[0].shape[0]
     if wp[0].shape[1] != k or k == 0 or rows == 0 or (act == "swiglu" and rows % 2):
@@ -1170,9 +1170,9 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     if out_dtype not in _LINEAR_OUT:
         raise SchemeError(f"dtype must be float32 or bfloat16, got {out_dtype}")
     x_op, w_op = _operand(xp, "x", False), _operand(wp, "w", False)
-    dx = torch.empty((toks, k), dtype=out_dtype, device=on)
-    dw = torch.empty((rows, k), dtype=out_dtype, device=on)
-    db = torch.empty(rows, dtype=torch.float32, device=on) if bias_grad else None
+    dx = empty((toks, k), dtype=out_dtype)
+    dw = empty((rows, k), dtype=out_dtype)
+    db = empty(rows, dtype=torch.float32) if bias_grad else None
     if toks == 0:
         dw.zero_()
         if db is not None:
@@ -1184,7 +1184,7 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     hi, lo, ldz = None, None, 0
     if not as_is:
         ldz = -(-rows // 8) * 8
-        hi = torch.empty((toks, ldz), dtype=torch.bfloat16, device=on)
+        hi = empty((toks, ldz), dtype=torch.bfloat16)
         # bf16 gradients: dz rounded as they are; the pair would double both
         # products.  A pair of operands keeps the float32-faithful form
         if out_dtype == torch.float32 or xp[1] is not None:
@@ -1192,7 +1192,8 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     scratch = None
     if bias_grad:
         nbytes = int(lib().mr_act_grad_workspace_bytes(toks, feats, code))
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=on)
+        if nbytes:
+            scratch = empty(nbytes, dtype=torch.uint8)
     if bias_grad or not as_is:
         z = None if act == "none" else pre.data_ptr()
         _launch("mr_act_grad", dev, dy.data_ptr(), DTYPES[dy.dtype], ldy, z, ldp, toks, feats, code,
