@@ -171,9 +171,9 @@ class ClockSampler:
                 "source": "nvml" if self.handle is not None else "nvidia-smi"}
 
 
-# DRAM bytes (read + write) per K3 launch, averaged over the 11 weight GEMMs of
-# one 7B step (16384 tokens, N=1, the tuning form: forward bf16x3, backward
-# tf32), from one ncu capture of each shape's warm launch:
+# DRAM bytes (read + write) per launch, averaged over the 11 weight GEMMs of one
+# 7B step (16384 tokens, N=1, the tuning form: forward bf16x3, backward tf32), all
+# on K3 (the forward's four launches are on K13 now), from one ncu capture of each shape's warm launch:
 #   ncu --metrics dram__bytes_read.sum,dram__bytes_write.sum,gpu__time_duration.sum
 #       --clock-control none -k regex:gemm_kernel --csv
 #       python -m mround_b200.kernel_sweep --gemm-all 16384
@@ -438,14 +438,15 @@ def main():
                    "l2": "inputs larger than L2 (235 MB per batch input)"},
         "ms_forward_batch": t_fwd, "block_seconds": blk_s, "wall_s_model": blk_s * arch.layers,
         "gpu_launches": launches,
-        "roofline": {"bound": "tensor", "kernel": "mround_b200 gemm_kernel (K3)",
+        "roofline": {"bound": "tensor",
+                     "kernel": "mround_b200 gemm_kernel (K3), linear_wide_kernel (K13)",
                      "achieved": achieved, "peak": peak, "unit": "TFLOP/s",
                      "frac": achieved / peak, "peak_source": peak_src,
                      "executed_tflops": exe_flops / (gemm_ms / 1e3) / 1e12 if gemm_ms else 0.0,
                      "executed_frac": (exe_flops / (gemm_ms / 1e3) / 1e12) / peak if gemm_ms else 0.0,
                      "gemm_share_of_step": gemm_ms / t_step if t_step else None,
                      "traffic": GEMM_TRAFFIC_7B if args.arch == "qwen2.5-7b" and dist.world == 1 else None,
-                     "traffic_unit": "bytes per weight-GEMM K3 launch (DRAM read + write), ncu capture of each shape"},
+                     "traffic_unit": "bytes per weight GEMM as a K3 launch (DRAM read + write), ncu capture of each shape"},
         "clocks": clocks.summary(),
         "e2e": e2e,
     }
