@@ -811,6 +811,11 @@ def _launch(name: str, dev: int, *args) -> None:
     LAUNCHES[0] += 1
 
 
+def _strides(t: torch.Tensor) -> list[int]:
+    """The strides that count: of dimensions with more than one element."""
+    return [stride for size, stride in zip(t.shape, t.stride()) if size > 1]
+
+
 def _dtype_code(t: torch.Tensor, name: str) -> int:
     code = DTYPES.get(t.dtype)
     if code is None:
@@ -846,6 +851,10 @@ def _rotary(q, k, cos, sin, positions, layout, out, transposed):
             if x is not None and (y.shape != x.shape or y.dtype != dtype):
                 raise SchemeError(f"an output is {tuple(y.shape)} {y.dtype}, expected "
                                   f"{tuple(x.shape)} {dtype}")
+            if x is not None and 0 in _strides(y):
+                raise SchemeError(f"an output's elements share storage, strides {y.stride()}")
+            if x is not None and y.data_ptr() == x.data_ptr() and _strides(y) != _strides(x):
+                raise SchemeError("an output in its input's storage must have its strides")
     yq, yk = out
     dev = _device_of("q k cos sin positions out_q out_k", q, k, cos, sin, positions, yq, yk)
     code = _dtype_code(q, "q")
@@ -1001,6 +1010,8 @@ def distill_topk_grad(logits, t_logits, t_index, *, temperature: float = 1.0, we
         if out.shape != logits.shape or out.dtype != logits.dtype:
             raise SchemeError(f"out must be {tuple(logits.shape)} {logits.dtype}")
         _, _, ldg = _logit_rows(out)
+        if out.data_ptr() == logits.data_ptr() and _strides(out) != _strides(logits):
+            raise SchemeError("out in the logits' storage must be the logits")
     _distill(logits, t_logits, t_index, temperature, weight, loss, out, (None, None), ldg)
     return loss, out
 
@@ -1126,10 +1137,15 @@ def linear(x, w, *, bias=None, act: str = "none", residual=None, out=None, dtype
         if dtype is not None and out.dtype != dtype:
             raise SchemeError(f"out is {out.dtype}, not {dtype}")
         ldo = _row_stride(out, toks, feats, _LINEAR_OUT, "out")
+        if out.data_ptr() in (xp[0].data_ptr(), wp[0].data_ptr()) and toks:
+            raise SchemeError("out must not be an operand's storage")
     if t32 is not None:
         if _row_stride(t32, toks, feats, (torch.float32,), "t32") != ldo:
             raise SchemeError("t32 must have the output's row stride")
     ldr = 0 if residual is None else _row_stride(residual, toks, feats, _LINEAR_OUT, "residual")
+    if residual is not None and residual.data_ptr() == out.data_ptr() and toks and (
+            ldr != ldo or residual.dtype != out.dtype):
+        raise SchemeError("a residual in out's storage must be out")
     ldp = 0 if pre is None else _row_stride(pre, toks, rows, (torch.float32,), "pre")
     if bias is not None:
         _ptr(bias, torch.float32, "bias", rows)

@@ -312,3 +312,11 @@ def test_refusals_on_the_device(K):
             bad()
     with pytest.raises(PlatformError):
         K.distill_topk(x, t.cpu(), i)
+
+
+@pytest.mark.gpu
+def test_refuses_a_gradient_that_overlays_the_logits_differently(K):
+    buf = torch.zeros(4, 16, device="cuda")
+    t, i = torch.zeros(2, 3, device="cuda"), torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    with pytest.raises(SchemeError, match="storage"):
+        K.distill_topk_grad(buf[:2, :8], t, i, out=buf.view(-1)[:16].view(2, 8))

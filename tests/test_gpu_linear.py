@@ -433,3 +433,59 @@ def test_gradients_of_a_plain_linear(K, T, F, k, dtype):
         off = (T / 4 + 8) * 2.0 ** -24 * dy.double().abs().sum(0)
         close(db, dy.double().sum(0), off, 2.0 ** -24)
         wide.fill_(math.nan)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "swiglu"])
+def test_activation_of_large_values(K, act, dtype):
+    """Far from zero an activation is z or nothing, without overflow on the way."""
+    z = torch.tensor([1e2, 1e4, 1e20, 3e38, math.inf], device="cuda").to(torch.bfloat16)
+    z = torch.cat([z, -z[:-1], torch.tensor([math.nan], device="cuda").to(torch.bfloat16)])
+    w = torch.zeros(16 if act == "swiglu" else 8, 8, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(z.numel(), 8, dtype=torch.bfloat16, device="cuda")
+    x[:, 0], x[:, 1] = z, 1
+    w[0, 0] = 1
+    if act == "swiglu":
+        w[8, 1] = 1
+    out = K.linear(x, w, act=act, dtype=dtype)[:, 0]
+    # swiglu's up row multiplies the infinity by its zero weight: 0 * inf is NaN
+    finite = 4 if act == "swiglu" else 5
+    assert torch.equal(out[:finite], z[:finite].to(dtype))
+    assert (out[5:9].float().abs() <= 2.0 ** -100).all() and out[9].isnan()
+
+
+@pytest.mark.gpu
+def test_refuses_outputs_in_operands(K):
+    x, w, g = make(32, 32, 32, "none", 1, 3)
+    buf = torch.zeros(32, 64, device="cuda")
+    for bad in (dict(out=x), dict(out=w),
+                dict(out=buf[:, :32], residual=buf.view(-1)[:1024].view(32, 32)),
+                dict(out=buf[:, :32], residual=buf.view(torch.bfloat16)[:, :32])):
+        with pytest.raises(SchemeError, match="storage"):
+            K.linear(x, w, **bad)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(K):
+    """Calls that overlap share nothing: the same results as one after another."""
+    cases = [make(T, F, 512, act, 1, i) + (act,)
+             for i, (T, F, act) in enumerate([(1, 4096, "silu"), (300, 700, "gelu"),
+                                              (2000, 1000, "swiglu")])]
+    def step(x, w, act):
+        pre = torch.empty(x.shape[0], w.shape[0], device="cuda")
+        y = K.linear(x, w, act=act, pre=pre)
+        return (y, *K.linear_bwd(y, x, w, act=act, pre=pre, bias_grad=True))
+
+    want = [step(x, w, act) for x, w, _, act in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([step(x, w, act) for x, w, _, act in cases])
+    torch.cuda.synchronize()
+    for run_ in got:
+        for a, b in zip(run_, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))

@@ -237,3 +237,18 @@ def test_refusals_on_the_device(K):
         K.rotary(q[..., :16], None, cos, sin)
     with pytest.raises(PlatformError):
         K.rotary(q, None, cos.cpu(), sin)
+
+
+@pytest.mark.gpu
+def test_refuses_shared_outputs(K):
+    """Outputs whose elements share storage, or overlay the input differently."""
+    cos, sin = rope_tables(8, 32, 1e4, "cuda")
+    q = torch.zeros(2, 4, 2, 32, device="cuda")
+    with pytest.raises(SchemeError, match="share storage"):
+        K.rotary(q, None, cos, sin, out=(q[:1].expand(2, 4, 2, 32), None))
+    with pytest.raises(SchemeError, match="strides"):
+        K.rotary(q, None, cos, sin, out=(q.view(2, 2, 4, 32).transpose(1, 2), None))
+    one = torch.ones(1, 1, 2, 32, device="cuda")  # strides of single positions do not count
+    again = one.as_strided((1, 1, 2, 32), (7, 5, 32, 1))
+    want = K.rotary(one, None, cos, sin)[0]
+    assert torch.equal(K.rotary(one, None, cos, sin, out=(again, None))[0], want)
