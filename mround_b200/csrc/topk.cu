@@ -433,10 +433,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) topk_kernel(const __grid_consta
     }
     __syncwarp();
     cluster_sync_all();
-    for (int i = 0; i < g.parts; ++i) {
-      floor_key = max(floor_key, ld_cluster_u32(map_rank(smem_u32(&sh.floor_key), i)));
-      over |= ld_cluster_u32(map_rank(smem_u32(&sh.over), i)) != 0;
-    }
+    // a lane per CTA: one remote access after another would cost as many latencies
+    const int from = lane < g.parts ? lane : 0;
+    const uint32_t theirs = ld_cluster_u32(map_rank(smem_u32(&sh.floor_key), from));
+    over = ld_cluster_u32(map_rank(smem_u32(&sh.over), from)) != 0;
+    floor_key = __reduce_max_sync(0xffffffffu, theirs);
+    over = __any_sync(0xffffffffu, over);
   }
   if (!over) {
     for (int i = lane; i < listed; i += 32) {
@@ -456,20 +458,25 @@ __global__ void __launch_bounds__(THREADS, CTAS) topk_kernel(const __grid_consta
   } else {
     __syncwarp();
     cluster_sync_all();  // every CTA's survivors are in place
+    const int theirs =
+        lane < g.parts ? int(ld_cluster_u32(map_rank(smem_u32(&sh.kept), lane))) : 0;
+    over |= __any_sync(0xffffffffu, theirs > kTopShort);
+    int end[8];  // of each CTA's survivors in the joint list
     total = 0;
-    for (int i = 0; i < g.parts; ++i) {
-      const int theirs = int(ld_cluster_u32(map_rank(smem_u32(&sh.kept), i)));
-      over |= theirs > kTopShort;
-      total += theirs;
-    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) end[i] = total += __shfl_sync(0xffffffffu, theirs, i);
     over |= total > sh.kList;
     if (!over) {
-      int at = 0;
-      for (int i = 0; i < g.parts; ++i) {
-        const int theirs = int(ld_cluster_u32(map_rank(smem_u32(&sh.kept), i)));
-        const uint32_t from = map_rank(smem_u32(sh.cut), i);
-        for (int j = tid; j < theirs; j += THREADS) sh.list[at + j] = ld_cluster_u64(from + j * 8u);
-        at += theirs;
+      for (int at = tid; at < total; at += THREADS) {
+        int from = 0, start = 0;
+#pragma unroll
+        for (int i = 0; i < 7; ++i) {
+          if (at >= end[i]) {
+            from = i + 1;
+            start = end[i];
+          }
+        }
+        sh.list[at] = ld_cluster_u64(map_rank(smem_u32(sh.cut), from) + uint32_t(at - start) * 8u);
       }
       all = sh.list;
     }
