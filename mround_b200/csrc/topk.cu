@@ -8,10 +8,12 @@
 // k-th largest value: each thread keeps the two largest of its steps' maxima,
 // each of the W warps finds the ceil(k / W)-th largest of its 64, and F is the
 // smallest of these -- at least k values are >= F, so what is below F cannot be
-// among the k largest.  Only a vector whose maximum reaches F is looked into;
-// values not below F go to the warp's list in shared memory, a lane's lowest
-// remaining column at a time.  (Each thread appending its own, unrolled, kept
-// the warps waiting for instructions: 133 us for 1024 x 152064 bf16.)  F is
+// among the k largest.  A step (four vectors a lane) whose maximum reaches F in
+// any lane of the warp is compared with F whole, two values an instruction, into
+// one mask per lane; values not below F go to the warp's list in shared memory,
+// one of each lane's at a time.  (1024 x 152064 bf16: each thread appending its
+// own, unrolled, kept the warps waiting for instructions, 133 us; vector by
+// vector 82; now 59 us, 5.3 TB/s of the 6.5 a copy reaches.)  F is
 // refreshed when the part read has doubled, so a row in no special order lists
 // little more than k values per doubling.  At the end the list is cut to the
 // last F, and each survivor's rank is the number of listed keys above it
@@ -21,10 +23,10 @@
 // Few rows are divided among the CTAs of a cluster: the largest of their F is
 // a bound for the whole row, and each ranks its survivors among everyone's.
 //
-// Of values equal to F a warp lists the first k only, so that a constant or
-// fully masked row costs no more than another.  A row whose list overflows all
-// the same (a rising row) takes the exact way instead: four 8-bit radix passes over the row
-// (from L2) find the k-th key and the number above it; the values above it, and
+// Of values equal to F a warp lists the first k only, counting them where they
+// come in numbers, so that a constant or fully masked row costs little more than
+// another.  A row whose list overflows all the same (a rising row) takes the
+// exact way instead: four 8-bit radix passes over the row (from L2) find the k-th key and the number above it; the values above it, and
 // the first columns equal to it, form the list.
 //
 // Results do not depend on the order in which threads append to the list.
@@ -41,7 +43,7 @@ namespace {
 
 constexpr int kTopUnroll = 4;     // 16-byte loads per thread and step
 constexpr int kTopWarpList = 512; // values a warp lists while streaming
-constexpr int kTopShort = 1280;   // of them, not below the last F
+constexpr int kTopShort = 1664;   // of them, not below the last F
 constexpr int kTopMaxK = 256;
 constexpr uint32_t kKeyLowest = 0x007FFFFFu;  // of -inf; empty slots are below
 
@@ -99,6 +101,87 @@ __device__ __forceinline__ float vec_max(const Vec16<T>& v) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
     const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
     return max_nan(__low2float(m), __high2float(m));
+  }
+}
+
+// The larger value in each half, NaN if either is.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
+  using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const P m = __hmax2_nan(*reinterpret_cast<const P*>(&a), *reinterpret_cast<const P*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+
+// The largest value of a step's vectors, NaN if they hold one.
+template <typename T>
+__device__ __forceinline__ float step_max(const Vec16<T> (&v)[kTopUnroll]) {
+  if constexpr (sizeof(T) == 4) {
+    float top = vec_max<T>(v[0]);
+#pragma unroll
+    for (int u = 1; u < kTopUnroll; ++u) top = max_nan(top, vec_max<T>(v[u]));
+    return top;
+  } else {  // pairs as long as there are several
+    Vec16<T> m = v[0];
+#pragma unroll
+    for (int u = 1; u < kTopUnroll; ++u) {
+      m.raw.x = pair_max<T>(m.raw.x, v[u].raw.x);
+      m.raw.y = pair_max<T>(m.raw.y, v[u].raw.y);
+      m.raw.z = pair_max<T>(m.raw.z, v[u].raw.z);
+      m.raw.w = pair_max<T>(m.raw.w, v[u].raw.w);
+    }
+    return vec_max<T>(m);
+  }
+}
+
+// Bit b: the value of word b & 15 of a step's vectors (its upper half for
+// b >= 16, of 2-byte types) is not below bar.
+template <typename T>
+__device__ __forceinline__ uint32_t not_below(const Vec16<T> (&v)[kTopUnroll], float bar) {
+  static_assert(kTopUnroll == 4, "16 words a step");
+  uint32_t below = 0;
+  auto each = [&](auto one) {
+#pragma unroll
+    for (int u = 0; u < kTopUnroll; ++u) {
+      below |= one(v[u].raw.x) << (4 * u) | one(v[u].raw.y) << (4 * u + 1) |
+               one(v[u].raw.z) << (4 * u + 2) | one(v[u].raw.w) << (4 * u + 3);
+    }
+  };
+  if constexpr (sizeof(T) == 4) {
+    each([&](uint32_t w) { return __uint_as_float(w) < bar ? 1u : 0u; });
+    return ~below & 0xFFFFu;
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 b = __half2half2(__float2half_ru(bar));  // the first value not below
+    each([&](uint32_t w) {
+      return __hlt2_mask(*reinterpret_cast<const __half2*>(&w), b) & 0x00010001u;
+    });
+    return ~below;
+  } else {
+    const __nv_bfloat162 b = __bfloat162bfloat162(__float2bfloat16_ru(bar));
+    each([&](uint32_t w) {
+      return __hlt2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w), b) & 0x00010001u;
+    });
+    return ~below;
+  }
+}
+
+// The value of bit b, and its column from the step's first one of this lane
+// (vectors `stride` columns apart).
+template <typename T>
+__device__ __forceinline__ float value_at(const Vec16<T> (&v)[kTopUnroll], int b, int stride,
+                                          int* col) {
+  const int u = b >> 2 & 3, q = b & 3;
+  const uint4 r = u < 2 ? (u == 0 ? v[0].raw : v[1].raw) : (u == 2 ? v[2].raw : v[3].raw);
+  const uint32_t w = q < 2 ? (q == 0 ? r.x : r.y) : (q == 2 ? r.z : r.w);
+  if constexpr (sizeof(T) == 4) {
+    *col = u * stride + q;
+    return __uint_as_float(w);
+  } else {
+    *col = u * stride + 2 * q + (b >> 4);
+    const uint16_t h = uint16_t(b & 16 ? w >> 16 : w);
+    if constexpr (std::is_same<T, __half>::value)
+      return __half2float(__ushort_as_half(h));
+    else
+      return bf16_to_f32(h);
   }
 }
 
@@ -313,6 +396,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) topk_kernel(const __grid_consta
   // are counted where they come in numbers only.
   float bar = -INFINITY;
   int ties = 0;
+  const int many = max(96, g.k + g.k / 2);  // listed: rows in no special order list fewer
   auto seen = [&](float m) {
     const uint32_t key = key_of(m);
     second = max(second, min(first, key));
@@ -358,16 +442,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) topk_kernel(const __grid_consta
   for (int step = 0; step < steps; ++step) {
     if (step + 1 < steps) load(ahead, step + 1);
     const int at = v0 + step * kStep + tid;
-    float m[kTopUnroll], top;
-#pragma unroll
-    for (int u = 0; u < kTopUnroll; ++u) {
-      m[u] = vec_max<T>(v[u]);
-      top = u ? max_nan(top, m[u]) : m[u];
-    }
+    const float top = step_max<T>(v);
     if (step == 0) {  // the first bound from every vector's maximum
 #pragma unroll
       for (int u = 0; u < kTopUnroll; ++u)
-        if (at + u * THREADS < v1) seen(m[u]);
+        if (at + u * THREADS < v1) seen(vec_max<T>(v[u]));
     } else if (at < v1) {
       seen(top);
     }
@@ -378,23 +457,26 @@ __global__ void __launch_bounds__(THREADS, CTAS) topk_kernel(const __grid_consta
     // out of order: these do not count as ties
     if (step == 0) list(loose, loose_col, loose_col >= 0 && !(loose < bar));
     if (__any_sync(0xffffffffu, !(top < bar))) {
+      uint32_t take = not_below<T>(v, bar);
+      if (step + 1 == steps) {  // vectors past the row's
 #pragma unroll
-      for (int u = 0; u < kTopUnroll; ++u) {
-        const int first_i = at - lane + u * THREADS;  // the warp's
-        unsigned int hits = __ballot_sync(0xffffffffu, first_i + lane < v1 && !(m[u] < bar));
-        if (!hits) continue;
-        unsigned int take = 0;  // of this lane's values
-        if (hits >> lane & 1u) {
-          float f[kN];
-          v[u].get(f);
+        for (int u = 0; u < kTopUnroll; ++u)
+          if (at + u * THREADS >= v1) take &= ~(0x000F000Fu << (4 * u));
+      }
+      if (listed > many || int(__reduce_add_sync(0xffffffffu, __popc(take))) > g.k - ties) {
+        // perhaps more equal to F than needed: column by column
 #pragma unroll
-          for (int j = 0; j < kN; ++j) take |= !(f[j] < bar) ? 1u << j : 0u;
-        }
-        if (__popc(hits) * kN > g.k - ties) {  // perhaps more equal to F than needed
+        for (int u = 0; u < kTopUnroll; ++u) {
+          unsigned int here = 0;  // this vector's, in the columns' order
+#pragma unroll
+          for (int j = 0; j < kN; ++j) {
+            const int b = sizeof(T) == 4 ? 4 * u + j : 4 * u + j / 2 + j % 2 * 16;
+            here |= (take >> b & 1u) << j;
+          }
           unsigned int same = 0;
 #pragma unroll 1
           for (int j = 0; j < kN; ++j)
-            same |= (take >> j & 1u) && pick<T>(v[u].raw, j) == floor_v ? 1u << j : 0u;
+            same |= (here >> j & 1u) && pick<T>(v[u].raw, j) == floor_v ? 1u << j : 0u;
           int before = __popc(same);
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
@@ -406,14 +488,22 @@ __global__ void __launch_bounds__(THREADS, CTAS) topk_kernel(const __grid_consta
           while (same && before + __popc(same) > g.k - ties) {  // the first columns' stay
             const unsigned int last = 1u << (31 - __clz(same));
             same ^= last;
-            take ^= last;
+            here ^= last;
           }
           ties += equal;  // this warp's later columns are above these
-          if (ties >= g.k && floor_v < INFINITY) bar = nextafterf(floor_v, INFINITY);
+          if (ties > g.k) ties = g.k;
+          while (__any_sync(0xffffffffu, here)) {  // each lane's lowest remaining one
+            const int j = __ffs(here) - 1;
+            list(pick<T>(v[u].raw, j & (kN - 1)), row.head + (at + u * THREADS) * kN + j, here != 0);
+            here &= here - 1;
+          }
         }
-        while (__any_sync(0xffffffffu, take)) {  // each lane's lowest remaining one
-          const int j = __ffs(take) - 1;
-          list(pick<T>(v[u].raw, j & (kN - 1)), row.head + (first_i + lane) * kN + j, take != 0);
+        if (ties >= g.k && floor_v < INFINITY) bar = nextafterf(floor_v, INFINITY);
+      } else {
+        while (__any_sync(0xffffffffu, take)) {  // one of each lane's
+          int col;
+          const float x = value_at<T>(v, __ffs(take) - 1, THREADS * kN, &col);
+          list(x, row.head + at * kN + col, take != 0);
           take &= take - 1;
         }
       }
