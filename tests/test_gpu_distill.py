@@ -82,6 +82,25 @@ def test_top_logits_of_awkward_rows(K, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", [(3, 40000, 64), (3, 40000, 200), (200, 9001, 40),
+                                      (160, 50257, 256), (2, 152064, 1)])
+def test_top_logits_of_few_levels(K, dtype, rows, n, k):
+    """Rows of few distinct values, the largest common or rare, early or late;
+    values of one type's smallest size, where the others are zero."""
+    g = torch.Generator(device="cuda").manual_seed(n + rows)
+    levels = torch.randint(0, 50, (rows, n), device="cuda", generator=g).float()
+    check_top(K, levels.to(dtype), k)
+    check_top(K, torch.randn(rows, n, device="cuda", generator=g).round().to(dtype), k)
+    rising = levels + torch.arange(n, device="cuda") // 1000
+    check_top(K, rising.to(dtype), k)
+    check_top(K, (-rising).to(dtype), k)
+    tiny = levels.to(dtype).mul_(torch.finfo(dtype).smallest_normal).div_(64)
+    assert (tiny > 0).any()
+    check_top(K, tiny, k)
+
+
+@pytest.mark.gpu
 def test_top_logits_of_strided_rows(K):
     """A column range of wider rows, off the 16-byte grid; the rest is not read."""
     g = torch.Generator(device="cuda").manual_seed(3)
