@@ -214,8 +214,8 @@ extern "C" int mr_act_grad(const void* dy, int dy_dtype, int64_t ldy, const floa
                            int64_t toks, int64_t feats, int act, uint16_t* hi, uint16_t* lo,
                            int64_t ldo, float* bias_grad, void* workspace, void* stream) {
   const int rows = act == MR_ACT_SWIGLU ? 2 : 1;
-  if (!dy || (!z && act != MR_ACT_NONE) || (!hi && (lo || !bias_grad)) || toks <= 0 || feats <= 0 || feats > 0x3fffffff ||
-      act < MR_ACT_NONE || act > MR_ACT_SWIGLU || ldy < feats || (z && ldz < rows * feats) ||
+  if (!dy || (!z && act != MR_ACT_NONE) || (!hi && (lo || !bias_grad)) || toks <= 0 ||
+      feats <= 0 || feats > 0x3fffffff || act < MR_ACT_NONE || act > MR_ACT_SWIGLU || ldy < feats || (z && ldz < rows * feats) ||
       (hi && ldo < rows * feats) || (dy_dtype != MR_F32 && dy_dtype != MR_BF16) ||
       strips_of(toks) > 65535)
     return MR_ERR_ARGUMENT;

@@ -26,8 +26,9 @@
 // Of values equal to F a warp lists the first k only, counting them where they
 // come in numbers, so that a constant or fully masked row costs little more than
 // another.  A row whose list overflows all the same (a rising row) takes the
-// exact way instead: four 8-bit radix passes over the row (from L2) find the k-th key and the number above it; the values above it, and
-// the first columns equal to it, form the list.
+// exact way instead: four 8-bit radix passes over the row (from L2) find the k-th
+// key and the number above it; the values above it, and the first columns equal
+// to it, form the list.
 //
 // Results do not depend on the order in which threads append to the list.
 

@@ -3,9 +3,9 @@
 The block is the mlx-lm Llama/Qwen2 decoder layer the reference runs in
 ``block_output`` (mround/pipeline/blocks.py:578-606), in float32 semantics.
 The tuning path (``forward_fused`` / ``backward_fused``) runs every op on this
-library's kernels -- the linears and the attention products on the tcgen05
-GEMMs (K3; K13 where a residual or SwiGLU follows), norms, RoPE, softmax and
-SwiGLU's backward on K7 -- with an explicit backward; ``DeviceBlock.forward`` is an autograd form (K3 linears, torch for
+library's kernels -- the forward's linears on K13, the other matrix products on
+K3, norms, RoPE, softmax and SwiGLU's backward on K7 and K10 -- with an explicit
+backward; ``DeviceBlock.forward`` is an autograd form (K3 linears, torch for
 the rest) kept as a cross-check:
 
     h1  = rmsnorm(x) * w_in            q|k|v = h1 @ Wqkv^T (+ b)

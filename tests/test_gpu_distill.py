@@ -5,8 +5,8 @@ n / 512 + 16 terms of 2**-22 relative error each, each addition 2**-24) and
 float64 beyond, so log q and q / q_ref - 1 are within
     e = (n / 512 + 16) * 2**-24 + 2**-21 + 3 * 2**-23 * max|x| / T
 (the last: the exponent (x - max) c takes three roundings, of the difference,
-of c = log2(e) / T and of the product, and the distance is at most 2 max|x|).  The loss is then within w T^2 e (sum p = 1), plus its own rounding;
-a gradient within w T (q e + 2**-24 p) plus half a step of its type.
+of c = log2(e) / T and of the product, and the distance is at most 2 max|x|).
+The loss is then within w T^2 e (sum p = 1), plus its own rounding; a gradient within w T (q e + 2**-24 p) plus half a step of its type.
 """
 
 from __future__ import annotations
@@ -207,7 +207,8 @@ def test_absent_repeated_and_masked_entries(K):
     # equal logits: q = 1 / 777 everywhere, and KL = sum p log p + log 777
     p = torch.softmax(t[5].double(), 0)
     want = (p * p.log()).sum() + math.log(777)
-    assert abs(loss[5].item() - want.item()) <= (777 / 512 + 16) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -24 * want.item()
+    off = (777 / 512 + 16) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -24 * want.item()
+    assert abs(loss[5].item() - want.item()) <= off
     assert torch.equal(x[5], x5) and torch.isnan(x4).all()
     i[6, 0] = 777                                # beyond the vocabulary: that row alone is NaN
     loss2, grad2 = K.distill_topk_grad(x, t, i, weight=w)

@@ -41,7 +41,8 @@ def product(x, w):
     for a, b in ((xl, wh), (xh, wl)):
         if a is None or b is None:
             continue
-        z, size, count = z + a.double() @ b.double().t(), size + a.double().abs() @ b.double().abs().t(), count + 1
+        z = z + a.double() @ b.double().t()
+        size, count = size + a.double().abs() @ b.double().abs().t(), count + 1
     return z, size, count
 
 
