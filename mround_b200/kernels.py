@@ -794,14 +794,17 @@ def _device_of(names: str, *tensors) -> int:
     return dev
 
 
-# the stream's handle alone: torch.cuda.current_stream() builds an object (3 us)
+# the stream's handle alone: torch.cuda.current_stream() builds an object (3 us).
+# Device and stream are asked for once a CUDA tensor is at hand, so the lazy
+# initialization that torch.cuda.current_device() checks for (1 us) has been.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _launch(name: str, dev: int, *args) -> None:
     """One C entry point on device ``dev``'s current stream (appended to ``args``)."""
     fn = getattr(lib(), name)
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         status = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -981,7 +984,7 @@ def distill_topk(logits, t_logits, t_index, *, temperature: float = 1.0, weight=
     occurs, one beyond the vocabulary makes its row NaN.  ``weight``: float32
     (rows,); a row of weight 0, or without an entry, gives 0 whatever it holds.
     Returns float32 (rows,)."""
-    loss = logits.new_empty(len(logits), dtype=torch.float32)
+    loss = logits.new_empty(logits.shape[:1], dtype=torch.float32)
     _distill(logits, t_logits, t_index, temperature, weight, loss, None, (None, None), 0)
     return loss
 
@@ -995,7 +998,7 @@ def distill_topk_grad(logits, t_logits, t_index, *, temperature: float = 1.0, we
     The gradient has the logits' type, in ``out`` when given (contiguous
     columns; ``logits`` itself may be given), or with ``split`` is the bf16
     (hi, lo) pair that :func:`gemm` takes.  Returns (loss, gradient)."""
-    loss = logits.new_empty(len(logits), dtype=torch.float32)
+    loss = logits.new_empty(logits.shape[:1], dtype=torch.float32)
     if split:
         if out is not None:
             raise SchemeError("a split gradient is allocated by the call")

@@ -344,7 +344,10 @@ def test_refusals():
     assert lib.mr_act_grad(p, 0, 8, None, 8, 4, 8, 1, p, p, 8, None, None, None) == -1
     assert lib.mr_act_grad(p, 2, 8, p, 8, 4, 8, 1, p, p, 8, None, None, None) == -1
     assert lib.mr_act_grad(p, 0, 8, p, 8, 65535 * 64 + 1, 8, 1, p, p, 8, None, None, None) == -1
-    assert lib.mr_act_grad(p, 0, 8, p, 8, 4, 8, 1, p, p, 8, p, None, None) == -6
+    assert lib.mr_act_grad_workspace_bytes(64, 8, 1) == 0  # one strip: none needed
+    assert lib.mr_act_grad(p, 0, 8, p, 8, 65, 8, 1, p, p, 8, p, None, None) == -6
+    assert lib.mr_act_grad(p, 0, 8, p, 8, 4, 8, 1, None, p, 8, None, None, None) == -1
+    assert lib.mr_act_grad(p, 0, 8, p, 8, 4, 8, 1, None, None, 8, None, None, None) == -1
 
 
 @pytest.mark.gpu
