@@ -8,11 +8,15 @@ runs only on the GPU: a CPU tensor is refused with ``PlatformError``.
 
 from __future__ import annotations
 
-from ctypes import addressof
-
 import torch
 
-from mround_b200._native import LinearOperand, RotaryHeads, check, lib
+from mround_b200._native import (
+    check,
+    lib,
+    pack_linear_operand,
+    pack_rotary_heads,
+    unpack_linear_operand,
+)
 from mround_b200.exceptions import PlatformError, SchemeError
 
 __all__ = [
@@ -826,7 +830,7 @@ def _dtype_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _rotary_heads(name: str, x, y, b: int, s: int, d: int, dtype) -> RotaryHeads:
+def _rotary_heads(name: str, x, y, b: int, s: int, d: int, dtype) -> bytes:
     """``mr_rotary_heads`` of the heads ``x``, turned into ``y`` (of x's shape)."""
     bx, px, heads, dx = x.shape
     if bx != b or px != s or dx != d or x.dtype != dtype or heads == 0:
@@ -836,7 +840,7 @@ def _rotary_heads(name: str, x, y, b: int, s: int, d: int, dtype) -> RotaryHeads
     yb, ys, yh, yd = y.stride()
     if (xd != 1 or yd != 1) and d > 1:
         raise SchemeError(f"{name}'s last dimension must be contiguous")
-    return RotaryHeads(x.data_ptr(), y.data_ptr(), xb, xs, xh, yb, ys, yh, heads)
+    return pack_rotary_heads(x.data_ptr(), y.data_ptr(), xb, xs, xh, yb, ys, yh, heads)
 
 
 def _rotary(q, k, cos, sin, positions, layout, out, transposed):
@@ -845,9 +849,11 @@ def _rotary(q, k, cos, sin, positions, layout, out, transposed):
         raise SchemeError("q and k are (batch, positions, heads, head dim)")
     b, s, _, d = q.shape
     dtype = q.dtype
+    given = ()
     if out is None:
         out = (torch.empty_like(q), None if k is None else torch.empty_like(k))
     else:
+        given = out
         for x, y in ((q, out[0]), (k, out[1])):
             if (x is None) != (y is None):
                 raise SchemeError("out is a (q, k) pair with k None exactly where k is")
@@ -859,7 +865,7 @@ def _rotary(q, k, cos, sin, positions, layout, out, transposed):
             if x is not None and y.data_ptr() == x.data_ptr() and _strides(y) != _strides(x):
                 raise SchemeError("an output in its input's storage must have its strides")
     yq, yk = out
-    dev = _device_of("q k cos sin positions out_q out_k", q, k, cos, sin, positions, yq, yk)
+    dev = _device_of("q k cos sin positions out_q out_k", q, k, cos, sin, positions, *given)
     code = _dtype_code(q, "q")
     if cos.dim() != 2 or cos.shape != sin.shape:
         raise SchemeError(f"cos and sin are (positions, rotated columns / 2) tables, got "
@@ -885,7 +891,7 @@ def _rotary(q, k, cos, sin, positions, layout, out, transposed):
     hq = _rotary_heads("q", q, yq, b, s, d, dtype)
     hk = None if k is None else _rotary_heads("k", k, yk, b, s, d, dtype)
     if b * s:
-        _launch("mr_rotary", dev, addressof(hq), None if hk is None else addressof(hk),
+        _launch("mr_rotary", dev, hq, hk,
                 _ptr(cos, torch.float32, "cos"), _ptr(sin, torch.float32, "sin"), rows, pos_ptr,
                 pos64, pos_stride, b, s, d, 2 * half, inter, transposed, code)
     return out
@@ -1053,7 +1059,7 @@ def _operand(parts, name: str, kmajor: bool):
     if (inner != 1 and cols > 1) or ld < cols or ld % 8:
         raise SchemeError(f"{name} needs contiguous columns and a row stride that is a multiple "
                           f"of 8, got strides {hi.stride()}")
-    return LinearOperand(hi.data_ptr(), None if lo is None else lo.data_ptr(), ld, kmajor)
+    return pack_linear_operand(hi.data_ptr(), 0 if lo is None else lo.data_ptr(), ld, kmajor)
 
 
 def _row_stride(t, rows: int, cols: int, dtypes, name: str) -> int:
@@ -1077,7 +1083,7 @@ def _linear_call(dev, x, w, toks, feats, k, act, bias, residual, ldr, out, lo, t
     if timing:
         start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         start.record()
-    _launch("mr_linear", dev, addressof(x), addressof(w), toks, feats, k, act,
+    _launch("mr_linear", dev, x, w, toks, feats, k, act,
             None if bias is None else bias.data_ptr(),
             None if residual is None else residual.data_ptr(),
             0 if residual is None else DTYPES[residual.dtype], ldr, out.data_ptr(),
@@ -1086,7 +1092,7 @@ def _linear_call(dev, x, w, toks, feats, k, act, bias, residual, ldr, out, lo, t
             ldp, splits)
     if timing:
         end.record()
-        products = 1 + (x.lo is not None) + (w.lo is not None)
+        products = 1 + sum(unpack_linear_operand(p)[1] != 0 for p in (x, w))
         GEMM_EVENTS.append((start, end, 2.0 * toks * feats * (2 if act == 4 else 1) * k, products))
 
 

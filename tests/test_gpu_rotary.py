@@ -252,3 +252,15 @@ def test_refuses_shared_outputs(K):
     again = one.as_strided((1, 1, 2, 32), (7, 5, 32, 1))
     want = K.rotary(one, None, cos, sin)[0]
     assert torch.equal(K.rotary(one, None, cos, sin, out=(again, None))[0], want)
+
+
+def test_packed_arguments():
+    """The bytes passed for a structure are the structure's."""
+    from mround_b200 import _native as n
+
+    heads = (1 << 40, 3 << 33, 5, 1 << 35, 7, 0, 11, 1 << 41, 13)
+    assert n.pack_rotary_heads(*heads) == bytes(n.RotaryHeads(*heads))
+    for operand in ((1 << 40, 3 << 33, 1 << 35, 1), (1 << 40, None, 8, 0)):
+        packed = n.pack_linear_operand(*(v or 0 for v in operand))
+        assert packed == bytes(n.LinearOperand(*operand))
+        assert n.unpack_linear_operand(packed) == tuple(v or 0 for v in operand)
