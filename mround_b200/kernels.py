@@ -1027,6 +1027,10 @@ def distill_topk_grad(logits, t_logits, t_index, *, temperature: float = 1.0, we
 
 ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "swiglu": 4}
 LINEAR_SPLITS = (1, 2, 4, 8)
+# Up to so many tokens and weights a linear's gradients are bound by their launches:
+# carrying dz as a pair costs the device 1 to 3 us of 15 to 35 that the host takes
+# anyway (896 x 4864, 128 tokens: 28.2 and 31.1), but 20 % of 18944 x 3584.
+DZ_PAIR_TOKENS, DZ_PAIR_WEIGHTS = 128, 1 << 23
 
 
 def _act_code(act: str) -> int:
@@ -1173,8 +1177,9 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     ``dx = dz @ w`` and ``dw = dz.T @ x``, ``dz = dy * act'(pre)``, are ``dtype``
     (float32 or bfloat16; by default as the output of :func:`linear`), the bias
     gradient float32.  ``dz`` is carried as a bf16 pair into float32 gradients,
-    and rounded to bf16 once, like them, into bfloat16 ones; a bfloat16 ``dy``
-    without an activation is taken as it is."""
+    and into bfloat16 ones of up to 128 tokens and 2^23 weights; into larger ones
+    rounded to bf16 once, like them.  A bfloat16 ``dy`` without an activation is
+    taken as it is."""
     code = _act_code(act)
     xp, wp = _parts(x, "x"), _parts(w, "w")
     dev = _device_of("dy x x_lo w w_lo pre", dy, *xp, *wp, pre)
@@ -1210,9 +1215,11 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     if not as_is:
         ldz = -(-rows // 8) * 8
         hi = empty((toks, ldz), dtype=torch.bfloat16)
-        # bf16 gradients: dz rounded as they are; the pair would double both
-        # products.  A pair of operands keeps the float32-faithful form
-        if out_dtype == torch.float32 or xp[1] is not None:
+        # bf16 gradients: dz rounded as they are, since the pair would double both
+        # products, unless they are small.  A pair of operands keeps the
+        # float32-faithful form
+        if out_dtype == torch.float32 or xp[1] is not None or (
+                toks <= DZ_PAIR_TOKENS and rows * k <= DZ_PAIR_WEIGHTS):
             lo = torch.empty_like(hi)
     scratch = None
     if bias_grad:
@@ -1226,9 +1233,11 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
                 None if db is None else db.data_ptr(),
                 None if scratch is None else scratch.data_ptr())
     n = splits or 0
-    dz = (dy, None) if as_is else (hi[:, :rows], None if lo is None else lo[:, :rows])
-    _linear_call(dev, _operand(dz, "dz", True), w_op, toks, k, rows, 0, None, None, 0, dx, None,
-                 None, k, None, 0, n)
-    _linear_call(dev, _operand(dz, "dz", False), x_op, rows, k, toks, 0, None, None, 0, dw, None,
-                 None, k, None, 0, n)
+    if as_is:
+        hi, ldz = dy, ldy if toks > 1 else -(-rows // 8) * 8
+    dz = (hi.data_ptr(), 0 if lo is None else lo.data_ptr(), ldz)
+    _linear_call(dev, pack_linear_operand(*dz, True), w_op, toks, k, rows, 0, None, None, 0, dx,
+                 None, None, k, None, 0, n)
+    _linear_call(dev, pack_linear_operand(*dz, False), x_op, rows, k, toks, 0, None, None, 0, dw,
+                 None, None, k, None, 0, n)
     return dx, dw, db
