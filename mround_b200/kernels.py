@@ -1189,6 +1189,8 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     if wp[0].shape[1] != k or k == 0 or rows == 0 or (act == "swiglu" and rows % 2):
         raise SchemeError(f"x {tuple(xp[0].shape)} and w {tuple(wp[0].shape)} are not the operands "
                           "of a linear")
+    if wp[1] is not None and xp[1] is None:
+        raise SchemeError("w is a (hi, lo) pair but x is not")
     feats = rows // 2 if act == "swiglu" else rows
     ldy = _row_stride(dy, toks, feats, _LINEAR_OUT, "dy")
     if pre is None and act != "none":

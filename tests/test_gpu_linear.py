@@ -376,6 +376,9 @@ def test_refusals_on_the_device(K):
         K.linear_bwd(z(4, 16), x, w, act="silu")
     with pytest.raises(SchemeError):
         K.linear_bwd(z(4, 15), x, w)
+    for dy in (z(4, 16), z(4, 16, dtype=torch.bfloat16)):
+        with pytest.raises(SchemeError, match="pair"):
+            K.linear_bwd(dy, x, (w, w))
     with pytest.raises(PlatformError):
         K.linear(x, w.cpu())
 
