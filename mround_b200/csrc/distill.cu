@@ -22,8 +22,12 @@
 //
 // Exponentials are 2^(c x - a), c = log2(e) / T, a = round(c max): one fused
 // rounding of the exponent, and every term uses the same a, so its rounding
-// cancels in q.  A maximum beyond +-1e30 (a row of the type's lowest value
-// among them) would overflow a: such rows are summed again as 2^((x - max) c).
+// cancels in q.  It has to be small for that: below |c max| = 2^24 the largest
+// term is 2^+-0.5, but at 2^31 it would be 2^+-64, and further out infinite or
+// nothing.  So a running maximum starts at -2^24 / c, below which a value adds
+// to the sum without becoming the maximum, and a row whose maximum is not
+// between these bounds (a row masked whole, say) is summed again as
+// 2^((x - max) c).
 // Sums are float32 per thread and joined in float64 in a fixed order; the K
 // terms, and the logarithms, are in float64, because the loss is a difference
 // of logarithms of size ~10.  The kept columns are corrected after the row is
@@ -40,7 +44,7 @@ namespace {
 
 constexpr int kDistUnroll = 4;
 constexpr int kDistMaxK = 256;
-constexpr float kFar = 1e30f;  // maxima beyond this are not multiplied by c
+constexpr float kFarExponent = 16777216.f;  // largest |c max| of the fused form
 
 struct DistShared {
   float m[32];           // per streaming warp
@@ -74,10 +78,11 @@ __device__ __forceinline__ double warp_add(double v) {
   return v;
 }
 
-// (max, sum of exponentials relative to it) of one thread's values; a maximum
-// below -kFar stands for none.
+// (max, sum of exponentials relative to it) of one thread's values.  The
+// maximum starts at `lowest`, whose exponent is small enough for the fused form.
 struct Online {
-  float m = -kFar, s = 0.f;
+  float m, s = 0.f;
+  __device__ __forceinline__ explicit Online(float lowest) : m(lowest) {}
   template <int N>
   __device__ __forceinline__ void add(const float (&f)[N], float c) {
     float top = f[0];
@@ -104,7 +109,7 @@ __device__ __forceinline__ void warp_join(float c, float* m, double* s) {
 
 // Joins every streaming thread's (m, s) over the CTA and the cluster, in a
 // fixed order.  Each round has slots of its own.  All threads of the cluster
-// call it; m is at least -kFar, or c is 0.
+// call it; |m c| is at most kFarExponent unless the sum is to be formed again.
 template <int kWarps>
 __device__ void join(DistShared& sh, int round, int parts, bool streams, float m, float s, float c,
                      float* top, double* total) {
@@ -278,7 +283,8 @@ struct DistArgs {
   const float* t_logits;
   const int64_t* t_index;
   double temperature, inv_temperature;
-  float c;  // log2(e) / T
+  float c;    // log2(e) / T
+  float far;  // kFarExponent / c
   const float* weight;
   float* loss;
   GradOut out;
@@ -320,7 +326,7 @@ __global__ void __launch_bounds__(THREADS + 32, CTAS)
   double total = 1.0;
   bool far = false;
   if (!zeros) {
-    Online on;
+    Online on(-g.far);
     if (!streams) {
       teacher(sh, row, g.n, g.t_logits + r * g.k, g.t_index + r * g.k, g.k,
               g.inv_temperature, c);
@@ -382,7 +388,7 @@ __global__ void __launch_bounds__(THREADS + 32, CTAS)
     }
     join<THREADS / 32>(sh, 0, g.parts, streams, on.m, on.s, c, &top, &total);
     zeros = sh.empty;
-    far = !(top > -kFar && top < kFar);
+    far = !(top > -g.far && top < g.far);
     if (far) {  // the maximum alone, then the sum relative to it
       float m = -INFINITY, s = 0.f;
       if (streams) {
@@ -591,6 +597,7 @@ extern "C" int mr_distill_topk(const void* logits, int64_t rows, int n, int64_t 
   g.temperature = temperature;
   g.inv_temperature = 1.0 / temperature;
   g.c = float(1.4426950408889634 / temperature);
+  g.far = kFarExponent / g.c;
   g.weight = weight;
   g.loss = loss;
   g.out = GradOut{grad, grad_hi, grad_lo};
