@@ -36,7 +36,9 @@ __device__ __forceinline__ float silu_grad(float z) {
 template <bool kRough>
 __device__ __forceinline__ float gelu_tanh_grad(float z) {
   const float s = logistic<kRough>(1.5957691216057308f * (z + 0.044715f * z * z * z));
-  return s * (1.f + z * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * z * z));
+  // s (1 - s) first: far from zero it is 0 where z^3, or z^2, is infinite
+  const float a = z * (s * (1.f - s)) * 1.5957691216057308f;
+  return s + (a + a * z * z * 0.134145f);
 }
 template <bool kRough>
 __device__ __forceinline__ float gelu_grad(float z) {

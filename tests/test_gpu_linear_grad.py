@@ -1,0 +1,45 @@
+"""The gradients of K13 where its activations are far out, and what they may not
+depend on."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def K():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from mround_b200 import kernels
+
+    return kernels
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "swiglu"])
+def test_slopes_of_large_values(K, act, dtype):
+    """Far from zero a slope is 1 or nothing, without overflow on the way; with
+    and without the bias gradient, which is that of each token alone here."""
+    z = torch.tensor([1e2, 1e4, 1e9, 1e13, 2e13, 1e18, 1e19, 1e20, 3e38], device="cuda")
+    z = torch.cat([z, -z])
+    n = z.numel()
+    up = z > 0
+    x = torch.ones(n, 8, device="cuda", dtype=torch.bfloat16)
+    dy = torch.ones(n, 1, device="cuda")
+    if act == "swiglu":  # silu(z) times 1: the gate's slope, and silu(z) for the up row
+        w = torch.zeros(2, 8, device="cuda", dtype=torch.bfloat16)
+        w[0, 0] = w[1, 1] = 1
+        pre = torch.stack([z, torch.ones_like(z)], 1).contiguous()
+    else:
+        w = torch.ones(1, 8, device="cuda", dtype=torch.bfloat16)
+        pre = z[:, None].contiguous()
+    for bias_grad in (True, False):
+        dx, _, _ = K.linear_bwd(dy, x, w, act=act, pre=pre, bias_grad=bias_grad, dtype=dtype)
+        assert torch.equal(dx[up, 0], torch.ones(n // 2, device="cuda", dtype=dtype))
+        assert (dx[~up, 0].float().abs() <= 2.0 ** -100).all()
+    for i in range(n):
+        _, _, db = K.linear_bwd(dy[i:i + 1], x[i:i + 1], w, act=act, pre=pre[i:i + 1],
+                                bias_grad=True, dtype=dtype)
+        assert db[0] == 1 if up[i] else abs(db[0]) <= 2.0 ** -100
