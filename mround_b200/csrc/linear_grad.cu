@@ -7,11 +7,8 @@
 // features by four token lanes.  Bias sums stay in float32 registers, are
 // joined in the block and written per strip; a second kernel adds the strips
 // in token order, so the result does not depend on timing.  2047 tokens by 11008
-// features, tanh GELU, bf16 dy and dz: 41 us, 4.4 TB/s; 8192 tokens 135 us, 5.3 TB/s.
+// features, tanh GELU, bf16 dy and dz: 51 us from cold caches, 3.5 TB/s.
 
-#include <type_traits>
-
-#include "linear.h"
 #include "rowtypes.cuh"
 
 namespace mr {
@@ -22,47 +19,36 @@ constexpr int kGradTokens = 64;    // tokens per strip
 constexpr int kGradFeatures = 256; // features per block
 
 // act'(z).  SiLU and the tanh GELU (z times the logistic function of 2u, u' as
-// below) take one exponential and one division.  With kRough (dz in bf16 alone,
-// 2^-8) the forms approximate: error at most 2^-14 of the terms.
-template <bool kRough>
-__device__ __forceinline__ float logistic(float v) {
-  return kRough ? __fdividef(1.f, 1.f + __expf(-v)) : 1.f / (1.f + expf(-v));
-}
-template <bool kRough>
+// below) take one exponential and one division.
+__device__ __forceinline__ float logistic(float v) { return 1.f / (1.f + expf(-v)); }
 __device__ __forceinline__ float silu_grad(float z) {
-  const float s = logistic<kRough>(z);
+  const float s = logistic(z);
   return s * (1.f + z * (1.f - s));
 }
-template <bool kRough>
 __device__ __forceinline__ float gelu_tanh_grad(float z) {
-  const float s = logistic<kRough>(1.5957691216057308f * (z + 0.044715f * z * z * z));
+  const float s = logistic(1.5957691216057308f * (z + 0.044715f * z * z * z));
   // s (1 - s) first: far from zero it is 0 where z^3, or z^2, is infinite
   const float a = z * (s * (1.f - s)) * 1.5957691216057308f;
   return s + (a + a * z * z * 0.134145f);
 }
-template <bool kRough>
 __device__ __forceinline__ float gelu_grad(float z) {
-  if (kRough) {
-    const float tail = gelu_tail(z);
-    return (z < 0.f ? tail : 1.f - tail) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
-  }
   return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
          z * 0.39894228040143268f * expf(-0.5f * z * z);
 }
 
 // d act'(a) for one token's values
-template <bool kRough, int V>
+template <int V>
 __device__ __forceinline__ void times_grad(int act, const float (&d)[V], float (&a)[V]) {
   auto each = [&](auto fn) {
 #pragma unroll
     for (int i = 0; i < V; ++i) a[i] = d[i] * fn(a[i]);
   };
   if (act == MR_ACT_SILU)
-    each(silu_grad<kRough>);
+    each(silu_grad);
   else if (act == MR_ACT_GELU)
-    each(gelu_grad<kRough>);
+    each(gelu_grad);
   else if (act == MR_ACT_GELU_TANH)
-    each(gelu_tanh_grad<kRough>);
+    each(gelu_tanh_grad);
   else
     each([](float) { return 1.f; });
 }
@@ -107,7 +93,7 @@ __device__ __forceinline__ void put_pair(uint16_t* hi, uint16_t* lo, int64_t at,
 // sums: (strips, features of dz) or NULL.  One token at a time and six blocks an
 // SM: more loads in flight per thread cost blocks, and took longer (51 us against
 // 37 for four tokens).
-template <typename T, int V, bool kGated, bool kRough>
+template <typename T, int V, bool kGated>
 __global__ void __launch_bounds__(kGradFeatures, 6) act_grad_kernel(
     const T* __restrict__ dy, int64_t ldy, const float* __restrict__ z, int64_t ldz,
     int64_t toks, int feats, int act, uint16_t* __restrict__ hi, uint16_t* __restrict__ lo,
@@ -129,7 +115,7 @@ __global__ void __launch_bounds__(kGradFeatures, 6) act_grad_kernel(
         load_row<float, V>(z + t * ldz + feats + f, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float s = logistic<kRough>(a[i]);
+          const float s = logistic(a[i]);
           const float gate = d[i] * b[i] * (s * (1.f + a[i] * (1.f - s)));
           b[i] = d[i] * (a[i] * s);
           a[i] = gate;
@@ -137,7 +123,7 @@ __global__ void __launch_bounds__(kGradFeatures, 6) act_grad_kernel(
         }
         if (hi) put_pair<V>(hi, lo, t * ldo + feats + f, b);
       } else if (z) {
-        times_grad<kRough>(act, d, a);
+        times_grad(act, d, a);
       } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) a[i] = d[i];
@@ -184,21 +170,12 @@ int launch_act_grad(const void* dy, int64_t ldy, const float* z, int64_t ldz, in
   const int units = (feats + V - 1) / V;
   const dim3 grid((units + kGradFeatures / 4 - 1) / (kGradFeatures / 4), unsigned(strips_of(toks)));
   const T* d = static_cast<const T*>(dy);
-  auto launch = [&](auto gated, auto rough) {
-    act_grad_kernel<T, V, decltype(gated)::value, decltype(rough)::value>
-        <<<grid, kGradFeatures, 0, stream>>>(d, ldy, z, ldz, toks, feats, act, hi, lo, ldo, sums);
-  };
-  const bool rough = !lo && !sums;  // a bias gradient is float32
-  if (act == MR_ACT_SWIGLU) {
-    if (rough)
-      launch(std::true_type(), std::true_type());
-    else
-      launch(std::true_type(), std::false_type());
-  } else if (rough) {
-    launch(std::false_type(), std::true_type());
-  } else {
-    launch(std::false_type(), std::false_type());
-  }
+  if (act == MR_ACT_SWIGLU)
+    act_grad_kernel<T, V, true><<<grid, kGradFeatures, 0, stream>>>(d, ldy, z, ldz, toks, feats, act,
+                                                                    hi, lo, ldo, sums);
+  else
+    act_grad_kernel<T, V, false><<<grid, kGradFeatures, 0, stream>>>(d, ldy, z, ldz, toks, feats,
+                                                                     act, hi, lo, ldo, sums);
   return launch_status();
 }
 
@@ -217,7 +194,8 @@ extern "C" int mr_act_grad(const void* dy, int dy_dtype, int64_t ldy, const floa
                            int64_t ldo, float* bias_grad, void* workspace, void* stream) {
   const int rows = act == MR_ACT_SWIGLU ? 2 : 1;
   if (!dy || (!z && act != MR_ACT_NONE) || (!hi && (lo || !bias_grad)) || toks <= 0 ||
-      feats <= 0 || feats > 0x3fffffff || act < MR_ACT_NONE || act > MR_ACT_SWIGLU || ldy < feats || (z && ldz < rows * feats) ||
+      feats <= 0 || feats > 0x3fffffff || act < MR_ACT_NONE || act > MR_ACT_SWIGLU ||
+      ldy < feats || (z && ldz < rows * feats) ||
       (hi && ldo < rows * feats) || (dy_dtype != MR_F32 && dy_dtype != MR_BF16) ||
       strips_of(toks) > 65535)
     return MR_ERR_ARGUMENT;

@@ -43,3 +43,25 @@ def test_slopes_of_large_values(K, act, dtype):
         _, _, db = K.linear_bwd(dy[i:i + 1], x[i:i + 1], w, act=act, pre=pre[i:i + 1],
                                 bias_grad=True, dtype=dtype)
         assert db[0] == 1 if up[i] else abs(db[0]) <= 2.0 ** -100
+
+
+def operands(T, F, k, act, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rows = 2 * F if act == "swiglu" else F
+    x = torch.randn(T, k, device="cuda", generator=g).bfloat16()
+    w = (torch.randn(rows, k, device="cuda", generator=g) / k ** 0.5).bfloat16()
+    dy = torch.randn(T, F, device="cuda", generator=g).bfloat16()
+    pre = torch.randn(T, rows, device="cuda", generator=g) * 2
+    return x, w, dy, pre
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "swiglu"])
+@pytest.mark.parametrize("T,F,k", [(5, 66, 40), (200, 515, 264)])
+def test_bias_gradient_changes_no_other(K, T, F, k, act, dtype):
+    """dx and dw are the same whether the bias gradient is asked for or not."""
+    x, w, dy, pre = operands(T, F, k, act, T)
+    dx, dw, _ = K.linear_bwd(dy, x, w, act=act, pre=pre, bias_grad=True, dtype=dtype)
+    dx1, dw1, none = K.linear_bwd(dy, x, w, act=act, pre=pre, dtype=dtype)
+    assert none is None and torch.equal(dx, dx1) and torch.equal(dw, dw1)
