@@ -1027,10 +1027,6 @@ def distill_topk_grad(logits, t_logits, t_index, *, temperature: float = 1.0, we
 
 ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "swiglu": 4}
 LINEAR_SPLITS = (1, 2, 4, 8)
-# Up to so many tokens and weights a linear's gradients are bound by their launches:
-# carrying dz as a pair costs the device 1 to 3 us of 15 to 35 that the host takes
-# anyway (896 x 4864, 128 tokens: 28.2 and 31.1), but 20 % of 18944 x 3584.
-DZ_PAIR_TOKENS, DZ_PAIR_WEIGHTS = 128, 1 << 23
 
 
 def _act_code(act: str) -> int:
@@ -1176,10 +1172,9 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
 
     ``dx = dz @ w`` and ``dw = dz.T @ x``, ``dz = dy * act'(pre)``, are ``dtype``
     (float32 or bfloat16; by default as the output of :func:`linear`), the bias
-    gradient float32.  ``dz`` is carried as a bf16 pair into float32 gradients,
-    and into bfloat16 ones of up to 128 tokens and 2^23 weights; into larger ones
-    rounded to bf16 once, like them.  A bfloat16 ``dy`` without an activation is
-    taken as it is."""
+    gradient float32.  ``dz`` is formed in float32 and carried into both products
+    as a bf16 pair (2^-16 of it is lost), whatever the gradients' type; a
+    bfloat16 ``dy`` without an activation is taken as it is."""
     code = _act_code(act)
     xp, wp = _parts(x, "x"), _parts(w, "w")
     dev = _device_of("dy x x_lo w w_lo pre", dy, *xp, *wp, pre)
@@ -1217,12 +1212,10 @@ def linear_bwd(dy, x, w, *, act: str = "none", pre=None, bias_grad: bool = False
     if not as_is:
         ldz = -(-rows // 8) * 8
         hi = empty((toks, ldz), dtype=torch.bfloat16)
-        # bf16 gradients: dz rounded as they are, since the pair would double both
-        # products, unless they are small.  A pair of operands keeps the
-        # float32-faithful form
-        if out_dtype == torch.float32 or xp[1] is not None or (
-                toks <= DZ_PAIR_TOKENS and rows * k <= DZ_PAIR_WEIGHTS):
-            lo = torch.empty_like(hi)
+        # one bf16 alone would halve both products' work (2047 x 11008 by 2048, tanh
+        # GELU: 176 us instead of 330), but err by 1.41 times the rounding of a bf16
+        # gradient itself
+        lo = torch.empty_like(hi)
     scratch = None
     if bias_grad:
         nbytes = int(lib().mr_act_grad_workspace_bytes(toks, feats, code))

@@ -65,3 +65,30 @@ def test_bias_gradient_changes_no_other(K, T, F, k, act, dtype):
     dx, dw, _ = K.linear_bwd(dy, x, w, act=act, pre=pre, bias_grad=True, dtype=dtype)
     dx1, dw1, none = K.linear_bwd(dy, x, w, act=act, pre=pre, dtype=dtype)
     assert none is None and torch.equal(dx, dx1) and torch.equal(dw, dw1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,F,k", [(128, 200, 136), (129, 200, 136), (300, 520, 264),
+                                   (100, 4104, 2056)])
+@pytest.mark.parametrize("act", ["none", "silu", "gelu_tanh", "swiglu"])
+def test_bf16_gradients_err_by_one_rounding(K, T, F, k, act):
+    """Gradients in bf16 are those in float32 rounded: dz is carried as a pair,
+    so that both come from the same sums.  float32 against 64 bits is tested
+    elsewhere."""
+    x, w, dy, pre = operands(T, F, k, act, T)
+    for d in (dy, dy.float() + 2.0 ** -10):  # of a float32 dy too
+        args = dict(act=act, pre=None if act == "none" else pre)
+        dx, dw, _ = K.linear_bwd(d, x, w, dtype=torch.float32, **args)
+        dx16, dw16, _ = K.linear_bwd(d, x, w, dtype=torch.bfloat16, **args)
+        assert torch.equal(dx16, dx.bfloat16()) and torch.equal(dw16, dw.bfloat16())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "gelu_tanh", "swiglu"])
+def test_gradient_of_a_token_does_not_depend_on_the_others(K, act):
+    """splits = 1 fixes the order of the sums, and the tokens' number no precision."""
+    x, w, dy, pre = operands(600, 330, 520, act, 7)
+    whole, _, _ = K.linear_bwd(dy, x, w, act=act, pre=pre, splits=1)
+    for n in (1, 16, 128, 129, 300):
+        some, _, _ = K.linear_bwd(dy[:n], x[:n], w, act=act, pre=pre[:n], splits=1)
+        assert torch.equal(some, whole[:n])
