@@ -145,26 +145,32 @@ struct LinEpilogue {
 // silu as the block's element-wise kernels compute it
 __device__ __forceinline__ float silu1(float g) { return g / (1.f + expf(-g)); }
 
-// Phi(-|z|) = t 2^(p(t) - z^2 log2(e) / 2) with t = 1 / (1 + |z| / 2) and p the
-// quartic of least largest error (fitted for |z| <= 13.2, where the tail leaves
-// float32's range): relative error 5.5e-5.
+// The activations for a bf16 result, without the exact division's branches: to
+// 2^-20 of |z|, and to 2^-13 of the value where that is smaller.  The branches,
+// unrolled over 32 tokens, made the epilogue longer than the products: 2047 x
+// 2048 by 11008 features take 92 us with an exactly divided tanh GELU, 70 us so,
+// 66 us without an activation.  Float32 results, and pairs, take the exact forms.
+__device__ __forceinline__ float silu_rough(float g) {
+  return __fdividef(g, 1.f + __expf(-g));
+}
+
+// Phi(-|z|) = t 2^(p(t) - z^2 log2(e) / 2), t = 1 / (1 + |z| / 2): the form of
+// erfc's Chebyshev fit in Press et al., Numerical Recipes (2nd edition, 6.2).  p
+// is our own fit, of degree 8 and least largest error for |z| <= 13.2, where the
+// tail leaves float32's range: 6.4e-7 of the tail with these rounded constants.
 __device__ __forceinline__ float gelu_tail(float z) {
   const float t = __fdividef(1.f, fmaf(0.5f, fabsf(z), 1.f));
-  float p = fmaf(0.375025481f, t, -1.147340059f);
-  p = fmaf(p, t, 0.711058915f);
-  p = fmaf(p, t, 1.383448601f);
-  p = fmaf(p, t, -2.322162628f);
+  float p = fmaf(0.102767207f, t, -0.193010613f);
+  p = fmaf(p, t, -0.514969468f);
+  p = fmaf(p, t, 1.905410767f);
+  p = fmaf(p, t, -1.959707379f);
+  p = fmaf(p, t, 0.271629959f);
+  p = fmaf(p, t, 0.261255383f);
+  p = fmaf(p, t, 1.452787995f);
+  p = fmaf(p, t, -2.326163054f);
   float power;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(power) : "f"(fmaf(-0.72134752f * z, z, p)));
   return t * power;
-}
-
-// The activations to 2^-14 of the value or better, for a result that is rounded
-// to bf16 at once (2^-8).  The exact forms' branches, unrolled over 32
-// tokens, made the epilogue longer than the products: 2047 x 2048 by 11008
-// features took 128 us with a tanh GELU, 64.5 us without.
-__device__ __forceinline__ float silu_rough(float g) {
-  return __fdividef(g, 1.f + __expf(-g));
 }
 
 __device__ __forceinline__ float gelu_rough(float z) {
@@ -210,7 +216,7 @@ template <bool kGated, int N>
 __device__ __forceinline__ void finish_run(const LinEpilogue& e, int f, int t0, int end,
                                            float (&v)[N], const float (&up)[N]) {
   if (f >= e.feats || t0 >= end) return;
-  const bool rough = e.out_dtype == MR_BF16 && !e.lo && !e.t32;  // bf16 alone is kept
+  const bool rough = e.out_dtype == MR_BF16 && !e.lo;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (!kGated) break;

@@ -92,3 +92,19 @@ def test_gradient_of_a_token_does_not_depend_on_the_others(K, act):
     for n in (1, 16, 128, 129, 300):
         some, _, _ = K.linear_bwd(dy[:n], x[:n], w, act=act, pre=pre[:n], splits=1)
         assert torch.equal(some, whole[:n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "silu", "gelu", "gelu_tanh", "swiglu"])
+@pytest.mark.parametrize("T,F,k", [(3, 70, 256), (300, 257, 192), (2100, 640, 520)])
+def test_tf32_copy_changes_no_other(K, T, F, k, act):
+    """out is the same whether its tf32 copy, or z, is asked for or not."""
+    x, w, _, pre = operands(T, F, k, act, T)
+    t32 = torch.empty(T, F, device="cuda")
+    for dtype in (torch.bfloat16, torch.float32):
+        out = K.linear(x, w, act=act, dtype=dtype)
+        assert torch.equal(K.linear(x, w, act=act, dtype=dtype, t32=t32), out)
+        assert torch.equal(K.linear(x, w, act=act, dtype=dtype, pre=pre), out)
+        # the copy is the value before its rounding to bf16, kept to 2^-11 of it
+        off = 2.0 ** -11 + (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24)
+        assert ((t32 - out.float()).abs() <= off * (1 + off) * t32.abs() + 2.0 ** -126).all()
