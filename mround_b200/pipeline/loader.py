@@ -86,6 +86,30 @@ def _rope_scaling(where: str, entry) -> RopeScaling | None:
                        **given)
 
 
+def _rope_entries(config: dict) -> dict[str, dict]:
+    """The configuration's rotary entries that are not empty: ``rope_scaling``,
+    and ``rope_parameters``, as which transformers >= 5 writes all rotary settings
+    ({"rope_type", "rope_theta", ...}) instead of top-level keys."""
+    entries = {}
+    for where in ("rope_scaling", "rope_parameters"):
+        entry = config.get(where)
+        if entry:
+            if not isinstance(entry, dict):
+                raise ArchitectureError(f"{where} {entry!r} is not a set of rotary settings")
+            entries[where] = entry
+    return entries
+
+
+def _stated_once(what: str, found: dict, default):
+    """The value of a setting from the places that state one; refused where they
+    disagree."""
+    values = list(found.values())
+    if any(v != values[0] for v in values[1:]):
+        raise ArchitectureError(f"the configuration states {what} more than once, differently: "
+                                + ", ".join(f"{v} in {where}" for where, v in found.items()))
+    return values[0] if values else default
+
+
 class _SafetensorsFile:
     """Header of one safetensors file; tensors come back as memory-mapped views."""
 
@@ -146,15 +170,14 @@ class CheckpointModel:
         if config.get("mlp_bias"):
             raise ArchitectureError("mlp_bias=true (biases on gate/up/down_proj) is not "
                                     "implemented by the device block")
-        # transformers >= 5 writes the rotary settings as ``rope_parameters``
-        # ({"rope_type", "rope_theta", ...}) instead of top-level keys
-        rope = config.get("rope_parameters") or {}
-        scaling = _rope_scaling("rope_scaling", config.get("rope_scaling"))
-        if scaling is None:
-            scaling = _rope_scaling("rope_parameters", rope)
-        theta = config.get("rope_theta")
-        if theta is None:
-            theta = rope.get("rope_theta", 10000.0)
+        rope = _rope_entries(config)
+        scaling = _stated_once("a rope scaling", {
+            where: _rope_scaling(where, entry) for where, entry in rope.items()
+            if "rope_type" in entry or "type" in entry}, None)
+        theta = _stated_once("rope_theta", {
+            where: float(entry["rope_theta"]) for where, entry in
+            {"the top level": config, **rope}.items() if entry.get("rope_theta") is not None},
+            10000.0)
         self._config = config
         heads = int(config["num_attention_heads"])
         hidden = int(config["hidden_size"])
@@ -165,7 +188,7 @@ class CheckpointModel:
             head_dim=int(config.get("head_dim") or hidden // heads),
             intermediate=int(config["intermediate_size"]), vocab=int(config["vocab_size"]),
             rms_eps=float(config.get("rms_norm_eps", 1e-6)),
-            rope_theta=float(theta),
+            rope_theta=theta,
             qkv_bias=family == "qwen2",
             tied=bool(config.get("tie_word_embeddings", False)),
             rope_scaling=scaling,
