@@ -45,6 +45,7 @@ def is_checkpoint_dir(path: str | Path) -> bool:
 
 # what each scaling's configuration has to state, and may state
 _ROPE_KEYS = {
+    "default": ((), ()),
     "linear": (("factor",), ()),
     "llama3": (("factor", "low_freq_factor", "high_freq_factor",
                 "original_max_position_embeddings"), ()),
@@ -55,30 +56,29 @@ _ROPE_KEYS = {
 
 def _rope_scaling(where: str, entry) -> RopeScaling | None:
     """The scaling that a configuration's ``rope_scaling`` or ``rope_parameters``
-    describes; None for the unscaled embedding.  Refused: a kind this block does
+    describes; None for the unscaled embedding.  Its theta and partial factor are
+    read apart, since other places may state them.  Refused: a kind this block does
     not compute, a key it would ignore, or a missing one (readers disagree on
     defaults)."""
-    if not entry:
-        return None
     kind = entry.get("rope_type", entry.get("type", "default"))
     said = f"{where} {entry} (rope_type {kind!r})"
-    if kind == "default":
-        return None
     if kind not in _ROPE_KEYS:
         raise ArchitectureError(f"{said} is not implemented by the device block")
     needed, optional = _ROPE_KEYS[kind]
     missing = [k for k in needed if entry.get(k) is None]
     if missing:
         raise ArchitectureError(f"{said} does not state {', '.join(missing)}")
-    known = {"rope_type", "type", "rope_theta", "original_max_position_embeddings", *needed,
-             *optional}
+    known = {"rope_type", "type", "rope_theta", "partial_rotary_factor",
+             "original_max_position_embeddings", *needed, *optional}
     # settings whose stated value is what the block does
-    same = {"partial_rotary_factor": 1.0, "truncate": True}
+    same = {"truncate": True, "factor": 1.0}
     unknown = sorted(k for k, v in entry.items()
                      if k not in known and v is not None and v != same.get(k))
     if unknown:
         raise ArchitectureError(f"{said}: {', '.join(unknown)} is not implemented by the device "
                                 "block")
+    if kind == "default":
+        return None
     given = {k: float(entry[k]) for k in (*needed, *optional)
              if k != "original_max_position_embeddings" and entry.get(k) is not None}
     original = entry.get("original_max_position_embeddings")
@@ -98,6 +98,20 @@ def _rope_entries(config: dict) -> dict[str, dict]:
                 raise ArchitectureError(f"{where} {entry!r} is not a set of rotary settings")
             entries[where] = entry
     return entries
+
+
+def _rotary_dim(config: dict, entries: dict[str, dict], head_dim: int) -> int | None:
+    """The rotated columns of a head that ``partial_rotary_factor`` leaves, None for
+    all of them."""
+    factor = _stated_once("partial_rotary_factor", {
+        where: float(entry["partial_rotary_factor"])
+        for where, entry in {"the top level": config, **entries}.items()
+        if entry.get("partial_rotary_factor") is not None}, 1.0)
+    if not 0.0 < factor <= 1.0:
+        raise ArchitectureError(f"partial_rotary_factor must be above 0 and at most 1, got {factor}")
+    # rounded down, but for the factor's own rounding: 26 / 46 of 46 columns are 26
+    columns = int(head_dim * factor + 1e-6)
+    return None if columns == head_dim else columns
 
 
 def _stated_once(what: str, found: dict, default):
@@ -171,9 +185,10 @@ class CheckpointModel:
             raise ArchitectureError("mlp_bias=true (biases on gate/up/down_proj) is not "
                                     "implemented by the device block")
         rope = _rope_entries(config)
+        scalings = {where: _rope_scaling(where, entry) for where, entry in rope.items()}
         scaling = _stated_once("a rope scaling", {
-            where: _rope_scaling(where, entry) for where, entry in rope.items()
-            if "rope_type" in entry or "type" in entry}, None)
+            where: found for where, found in scalings.items()
+            if "rope_type" in rope[where] or "type" in rope[where]}, None)
         theta = _stated_once("rope_theta", {
             where: float(entry["rope_theta"]) for where, entry in
             {"the top level": config, **rope}.items() if entry.get("rope_theta") is not None},
@@ -181,18 +196,20 @@ class CheckpointModel:
         self._config = config
         heads = int(config["num_attention_heads"])
         hidden = int(config["hidden_size"])
+        head_dim = int(config.get("head_dim") or hidden // heads)
         self.arch = Arch(
             name=self.path.name, family=family, hidden=hidden,
             layers=int(config["num_hidden_layers"]), heads=heads,
             kv_heads=int(config.get("num_key_value_heads", heads)),
-            head_dim=int(config.get("head_dim") or hidden // heads),
+            head_dim=head_dim,
             intermediate=int(config["intermediate_size"]), vocab=int(config["vocab_size"]),
             rms_eps=float(config.get("rms_norm_eps", 1e-6)),
             rope_theta=theta,
             qkv_bias=family == "qwen2",
             tied=bool(config.get("tie_word_embeddings", False)),
             rope_scaling=scaling,
-            rope_interleaved=bool(config.get("rope_traditional", False)))
+            rope_interleaved=bool(config.get("rope_traditional", False)),
+            rotary_dim=_rotary_dim(config, rope, head_dim))
         self._files: dict[str, _SafetensorsFile] = {}
         self._where: dict[str, str] = {}
         index = self.path / "model.safetensors.index.json"
