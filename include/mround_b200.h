@@ -458,8 +458,9 @@ int mr_gemm_tile_n(int64_t m, int64_t n, int64_t k, int64_t batch, int precision
 int mr_gemm_tile_m(int64_t m, int64_t n, int64_t k, int64_t batch, int precision, int a_kmajor,
                    int b_kmajor, int causal);
 
-/* Device status word of K3 and K13: 0, or MR_ERR_TIMEOUT.  Synchronizes the
- * device; reset != 0 clears it. */
+/* Device status word of K3 and K13: 0, or MR_ERR_TIMEOUT once a wait gave up,
+ * from which moment on that kernel's products leave their outputs unwritten until
+ * the word is cleared (reset != 0).  Synchronizes the device. */
 int mr_gemm_status(int reset);
 
 /*
@@ -642,7 +643,8 @@ int mr_distill_topk(const void* logits, int64_t rows, int n, int64_t ld, int dty
  * the device (fewer rounding steps in one order per divisor, all of them
  * reproducible); 1, 2, 4, 8 fix the divisor.  With splits = 1 a token's
  * result does not depend on the other tokens of the call.  Device-side waits
- * are bounded; a wait that gives up is reported by mr_gemm_status.
+ * are bounded; a wait that gives up leaves the outputs unwritten, of this call and
+ * of later ones, and is reported by mr_gemm_status alone.
  */
 enum {
   MR_ACT_NONE = 0,

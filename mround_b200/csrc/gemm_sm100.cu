@@ -899,7 +899,9 @@ extern "C" int mr_gemm_tile_m(int64_t m, int64_t n, int64_t k, int64_t batch, in
 // after a wait gave up).  Synchronizes the device; `reset` clears the words.
 extern "C" int mr_gemm_status(int reset) {
   int v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(int));
+  // work on every stream: the copy alone waits for blocking ones
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(int));
   if (e != cudaSuccess) {
     set_cuda_error(e);
     return MR_ERR_LAUNCH;

@@ -17,10 +17,11 @@ from mround_b200._native import (
     pack_rotary_heads,
     unpack_linear_operand,
 )
-from mround_b200.exceptions import PlatformError, SchemeError
+from mround_b200.exceptions import DeviceError, PlatformError, SchemeError
 
 __all__ = [
     "LossWorkspace",
+    "check_products",
     "colsumsq_split",
     "deltaloss",
     "distill_topk",
@@ -403,6 +404,22 @@ def gemm(a_hi, a_lo, b_hi, b_lo, c, *, m: int, n: int, k: int, a_kmajor: bool, b
     if timing:
         end.record()
         GEMM_EVENTS.append((start, end, 2.0 * m * n * k, precision))
+
+
+def check_products(device=None) -> None:
+    """Raise :class:`DeviceError` if a matrix product of ``device`` (the current one
+    when None) gave up a wait, and clear the report.  Synchronizes the device.
+
+    The products (:func:`gemm` and its relatives, :func:`linear`,
+    :func:`linear_bwd`) wait for at most 2 s at a time inside the kernel.  One that
+    gives up writes nothing, nor do later ones of its kind, and no launch reports
+    it: whoever keeps their results calls this first, as tuning does before a block
+    is handed on and scoring before its scores are."""
+    with torch.cuda.device(device):
+        status = int(lib().mr_gemm_status(1))
+    if status:
+        raise DeviceError("a matrix product gave up waiting on the device; results since the last "
+                          f"check are not valid (status {status})")
 
 
 def gemm_rs(a_hi, a_lo, b_hi, b_lo, *, m: int, n: int, k: int, a_kmajor: bool, b_kmajor: bool,
@@ -1116,7 +1133,10 @@ def linear(x, w, *, bias=None, act: str = "none", residual=None, out=None, dtype
 
     ``splits``: how many CTAs share the k of one output tile (1, 2, 4 or 8),
     chosen by size when None.  It fixes the order of the sums: with 1 a token's
-    result is the same whatever other tokens are in the call."""
+    result is the same whatever other tokens are in the call.
+
+    A wait inside the kernel that gives up leaves the output unwritten;
+    :func:`check_products` raises for it."""
     code = _act_code(act)
     xp, wp = _parts(x, "x"), _parts(w, "w")
     dev = _device_of("x x_lo w w_lo bias residual out t32 pre", *xp, *wp, bias, residual, out, t32,

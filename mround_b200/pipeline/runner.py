@@ -28,6 +28,7 @@ from typing import Any
 
 import torch
 
+from mround_b200 import kernels
 from mround_b200.exceptions import ArchitectureError, CalibrationError, ResumeError
 from mround_b200.pipeline.block import TUNING_PRECISION, DeviceBlock, Precision
 from mround_b200.pipeline.dist import DistContext
@@ -376,6 +377,7 @@ class QuantizationRunner:
             layers = tuner.commit(self.keep_codes)
         torch.cuda.synchronize(self.device)
         tuner.close()
+        kernels.check_products(self.device)  # before the block is recorded or exported
         exported = {f"{name}.{p}": q for p, q in layers.items()}
         result = BlockResult(
             index=block.index, name=name, initial_loss=outcome["initial"],

@@ -98,6 +98,7 @@ def capture_top_logits(model, batches: Sequence[np.ndarray], k: int, *,
     for inp, x in zip(inputs, streams):
         hi, lo, _, _ = kernels.rmsnorm_split(x.view(-1, arch.hidden), norm, arch.rms_eps)
         found.append(kernels.topk_logits(_head_logits((hi, lo), head, *inp.shape), k))
+    kernels.check_products(dev)
     return found
 
 
@@ -301,7 +302,7 @@ def score_widths(model: SyntheticModel, batches: Sequence[np.ndarray], widths: S
         if distills:
             for value in losses.values():
                 dist.all_reduce_(value)
-    torch.cuda.synchronize(dev)
+    kernels.check_products(dev)
     for blk in blocks:
         for layer in blk.layers.values():
             layer.grad_ready.clear()
