@@ -560,7 +560,8 @@ int mr_peer_status(int reset);
  * p = positions[b * pos_stride + s] (int64 when positions64, else int32), or s
  * when positions is NULL; a position outside [0, table_rows) writes NaN to the
  * rotated columns.  q and k (k may be NULL) describe heads of d columns
- * (columns contiguous, the other strides in elements); y may be x.
+ * (columns contiguous, the other strides in elements); y may be x, and shares no
+ * other storage with what is read.
  * 1 <= d <= 1024, r even, 2 <= r <= d.  Any alignment of the element type;
  * 16-byte aligned data and strides take 16-byte accesses.
  */
@@ -615,7 +616,8 @@ int mr_topk_logits(const void* logits, int64_t rows, int n, int64_t ld, int k, i
  * gives NaN in that row.  weight NULL: 1.  logits (rows, n), row stride ld, of
  * `dtype`.  Outputs, any may be NULL: loss float32 (rows); the gradient either
  * as `dtype` in grad (may be logits itself, with ldg = ld) or as a bf16 pair
- * grad_hi / grad_lo, row stride ldg.  1 <= k <= 256, 1e-3 <= temperature <= 1e3.
+ * grad_hi / grad_lo, row stride ldg; it shares no other storage with what is read.
+ * 1 <= k <= 256, 1e-3 <= temperature <= 1e3.
  */
 int mr_distill_topk(const void* logits, int64_t rows, int n, int64_t ld, int dtype,
                     const float* t_logits, const int64_t* t_index, int k, double temperature,
@@ -638,7 +640,8 @@ int mr_distill_topk(const void* logits, int64_t rows, int n, int64_t ld, int dty
  * MR_BF16, row stride ldr, may be out's storage, or NULL.  out: MR_F32 or
  * MR_BF16, row stride ldo; out_lo (with MR_BF16): the bf16 part out leaves;
  * out_t32: the value rounded to tf32; pre: z in float32 (toks, rows of w), row
- * stride ldp, for mr_act_grad -- each may be NULL.
+ * stride ldp, for mr_act_grad -- each may be NULL.  None shares other storage
+ * with an operand, the bias, the residual or another output.
  * splits: 0 lets the call divide k among 1, 2, 4 or 8 CTAs where that fills
  * the device (fewer rounding steps in one order per divisor, all of them
  * reproducible); 1, 2, 4, 8 fix the divisor.  With splits = 1 a token's

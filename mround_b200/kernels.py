@@ -8,6 +8,8 @@ runs only on the GPU: a CPU tensor is refused with ``PlatformError``.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from mround_b200._native import (
@@ -840,6 +842,70 @@ def _strides(t: torch.Tensor) -> list[int]:
     return [stride for size, stride in zip(t.shape, t.stride()) if size > 1]
 
 
+@functools.lru_cache(maxsize=1024)
+def _extent(shape, stride, size: int) -> int:
+    """Bytes from a layout's first element to behind its last."""
+    return (sum((n - 1) * s for n, s in zip(shape, stride)) + 1) * size if 0 not in shape else 0
+
+
+def _meet(a, b, size_a: int, size_b: int, shift: int) -> bool:
+    """Whether two layouts, the second's first byte ``shift`` after the first's, may
+    share a byte.  Dimensions are (stride in bytes, extent), largest stride first.
+    A stride that both step by is taken out, and what is left of both compared
+    within one period; False is certain, True is not where the strides differ."""
+    span_a = sum(s * (n - 1) for s, n in a) + size_a
+    span_b = sum(s * (n - 1) for s, n in b) + size_b
+    if shift >= span_a or -shift >= span_b:
+        return False
+    period = max(a[0][0] if a else 0, b[0][0] if b else 0)
+    if period == 0:
+        return True
+    rest_a = a[1:] if a and a[0][0] == period else a
+    rest_b = b[1:] if b and b[0][0] == period else b
+    if (sum(s * (n - 1) for s, n in rest_a) + size_a > period
+            or sum(s * (n - 1) for s, n in rest_b) + size_b > period):
+        return True
+    shift %= period
+    return (_meet(rest_a, rest_b, size_a, size_b, shift)
+            or _meet(rest_a, rest_b, size_a, size_b, shift - period))
+
+
+@functools.lru_cache(maxsize=1024)
+def _layouts_meet(shape_a, stride_a, size_a: int, shape_b, stride_b, size_b: int,
+                  shift: int) -> bool:
+    dims = [sorted(((s * size, n) for n, s in zip(shape, stride) if n > 1 and s), reverse=True)
+            for shape, stride, size in ((shape_a, stride_a, size_a), (shape_b, stride_b, size_b))]
+    return _meet(*dims, size_a, size_b, shift)
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses of a tensor's first byte and of the one behind its last."""
+    at = t.data_ptr()
+    return at, at + (t.nbytes if t.is_contiguous() else
+                     _extent(t.shape, t.stride(), t.element_size()))
+
+
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors are the same elements in the same order."""
+    return (a is b or (a.data_ptr() == b.data_ptr() and a.dtype == b.dtype
+                       and _strides(a) == _strides(b)))
+
+
+def _check_apart(name: str, written: torch.Tensor, names: str, *read) -> None:
+    """Refuse a tensor to write that may share bytes with one that is read (None
+    apart).  Columns of one buffer beside each other share none, though their
+    address ranges interleave."""
+    first, end = _span(written)
+    for i, t in enumerate(read):
+        if t is None:
+            continue
+        at, behind = _span(t)
+        if (first < behind and at < end and first < end and at < behind and
+                _layouts_meet(written.shape, written.stride(), written.element_size(), t.shape,
+                              t.stride(), t.element_size(), at - first)):
+            raise SchemeError(f"{name} shares storage with {names.split()[i]}")
+
+
 def _dtype_code(t: torch.Tensor, name: str) -> int:
     code = DTYPES.get(t.dtype)
     if code is None:
@@ -907,6 +973,14 @@ def _rotary(q, k, cos, sin, positions, layout, out, transposed):
         raise SchemeError(f"{s} positions but tables of {rows} rows")
     hq = _rotary_heads("q", q, yq, b, s, d, dtype)
     hk = None if k is None else _rotary_heads("k", k, yk, b, s, d, dtype)
+    if given and b * s:
+        # in place, each output is exactly its own input
+        q_in, k_in = _same(yq, q), k is not None and _same(yk, k)
+        _check_apart("out's q", yq, "q k cos sin positions", None if q_in else q, k, cos, sin,
+                     positions)
+        if k is not None:
+            _check_apart("out's k", yk, "k q cos sin positions out's-q", None if k_in else k,
+                         None if q_in and k_in else q, cos, sin, positions, None if q_in else yq)
     if b * s:
         _launch("mr_rotary", dev, hq, hk,
                 _ptr(cos, torch.float32, "cos"), _ptr(sin, torch.float32, "sin"), rows, pos_ptr,
@@ -925,7 +999,8 @@ def rotary(q, k, cos, sin, *, positions=None, layout: str = "half", out=None):
     (j, j + r/2) for "half", (2j, 2j + 1) for "interleaved".  ``positions``:
     int32 or int64 (S,) or (B, S) table rows, 0..S-1 by default; a position
     outside the tables gives NaN.  ``out``: a (q, k) pair of tensors to write,
-    which may be ``q`` and ``k`` themselves.  Returns (q, k) turned."""
+    which may be ``q`` and ``k`` themselves, and share no other storage with what
+    is read.  Returns (q, k) turned."""
     return _rotary(q, k, cos, sin, positions, layout, out, 0)
 
 
@@ -1036,8 +1111,9 @@ def distill_topk_grad(logits, t_logits, t_index, *, temperature: float = 1.0, we
         if out.shape != logits.shape or out.dtype != logits.dtype:
             raise SchemeError(f"out must be {tuple(logits.shape)} {logits.dtype}")
         _, _, ldg = _logit_rows(out)
-        if out.data_ptr() == logits.data_ptr() and _strides(out) != _strides(logits):
-            raise SchemeError("out in the logits' storage must be the logits")
+        if logits.shape[0]:
+            _check_apart("out", out, "logits t_logits t_index weight",
+                         None if _same(out, logits) else logits, t_logits, t_index, weight)
     _distill(logits, t_logits, t_index, temperature, weight, loss, out, (None, None), ldg)
     return loss, out
 
@@ -1129,7 +1205,8 @@ def linear(x, w, *, bias=None, act: str = "none", residual=None, out=None, dtype
     or with ``split`` a bf16 (hi, lo) pair.  ``t32``: a contiguous float32
     tensor that also receives the output rounded to tf32.  ``pre``: a float32
     (T, features) tensor that receives ``x @ w.T + bias``, for
-    :func:`linear_bwd`.
+    :func:`linear_bwd`.  ``out`` or ``t32`` may be ``residual``; what is written
+    shares no other storage with what is read, or with one another.
 
     ``splits``: how many CTAs share the k of one output tile (1, 2, 4 or 8),
     chosen by size when None.  It fixes the order of the sums: with 1 a token's
@@ -1153,6 +1230,7 @@ def linear(x, w, *, bias=None, act: str = "none", residual=None, out=None, dtype
         raise SchemeError(f"splits must be one of {LINEAR_SPLITS}, got {splits}")
     feats = rows // 2 if act == "swiglu" else rows
     lo, ldo = None, feats
+    given = out is not None
     if split:
         if out is not None or dtype is not None:
             raise SchemeError("a split output is allocated by the call")
@@ -1166,19 +1244,23 @@ def linear(x, w, *, bias=None, act: str = "none", residual=None, out=None, dtype
         if dtype is not None and out.dtype != dtype:
             raise SchemeError(f"out is {out.dtype}, not {dtype}")
         ldo = _row_stride(out, toks, feats, _LINEAR_OUT, "out")
-        if out.data_ptr() in (xp[0].data_ptr(), wp[0].data_ptr()) and toks:
-            raise SchemeError("out must not be an operand's storage")
     if t32 is not None:
         if _row_stride(t32, toks, feats, (torch.float32,), "t32") != ldo:
             raise SchemeError("t32 must have the output's row stride")
     ldr = 0 if residual is None else _row_stride(residual, toks, feats, _LINEAR_OUT, "residual")
-    if residual is not None and residual.data_ptr() == out.data_ptr() and toks and (
-            ldr != ldo or residual.dtype != out.dtype):
-        raise SchemeError("a residual in out's storage must be out")
     ldp = 0 if pre is None else _row_stride(pre, toks, rows, (torch.float32,), "pre")
     if bias is not None:
         _ptr(bias, torch.float32, "bias", rows)
     if toks:
+        for name, written in (("out", out if given else None), ("t32", t32), ("pre", pre)):
+            if written is not None:
+                # of what is read, out or t32 may be the residual
+                _check_apart(name, written, "x x_lo w w_lo bias residual out t32", *xp, *wp, bias,
+                             None if residual is None or (written is not pre
+                                                          and _same(written, residual))
+                             else residual,
+                             out if given and written is not out else None,
+                             t32 if written is pre else None)
         _linear_call(dev, _operand(xp, "x", True), _operand(wp, "w", True), toks, feats, k, code,
                      bias, residual, ldr, out, lo, t32, ldo, pre, ldp, splits or 0)
     return (out, lo) if split else out
