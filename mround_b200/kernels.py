@@ -714,7 +714,8 @@ def heads_split(src, b: int, s: int, h: int, d: int, *, merge: bool, t32: bool =
 
 
 def swiglu_split(gu, t: int, i: int, *, t32: bool = False):
-    """silu(g) * u as (hi, lo, tf32 copy or None)."""
+    """silu(g) * u as (hi, lo, tf32 copy or None), from a gate|up that is at hand;
+    the block's forward has it from the epilogue of :func:`linear`, bit for bit."""
     hi, lo = _pair((t, i), gu.device)
     tt = _t32((t, i), gu.device, t32)
     st = lib().mr_swiglu_split(_ptr(gu, torch.float32, "gu", t * 2 * i), t, i, hi.data_ptr(),
@@ -790,7 +791,9 @@ def softmax_bwd_split(dp, p, rows: int, s: int, scale: float, band: bool = False
 
 # ------------------------------------------------- rotary, logits and linear operators
 # Unlike the functions above, these take tensors of any CUDA device and launch
-# on that device's current stream.
+# on that device's current stream.  Like them they are not recorded by autograd: an
+# input that requires a gradient gives an output that does not, and the gradients
+# are what the *_bwd and *_grad functions return.
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 

@@ -331,10 +331,11 @@ class DeviceBlock:
 # Saved for the backward: the operand splits, P (float32 and hi/lo), h, gu,
 # and the second norm's rstd.
 
-def _mm(a, b, c, *, m, n, k, a_kmajor, b_kmajor, lda, ldb, prec, bias=None, accumulate=False):
+
+def _mm(a, b, c, *, m, n, k, a_kmajor, b_kmajor, lda, ldb, prec):
     kernels.gemm(a[0], a[1] if prec >= 2 else None, b[0], b[1] if prec == 3 else None, c, m=m, n=n,
                  k=k, a_kmajor=a_kmajor, b_kmajor=b_kmajor, lda=lda, ldb=ldb, ldc=n,
-                 precision=prec, bias=bias, accumulate=accumulate)
+                 precision=prec)
 
 
 def _bmm(a, b, c, *, m, n, k, batch, a_kmajor, b_kmajor, lda, ldb, sa, sb, sc, causal=0, seq=0):
