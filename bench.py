@@ -172,13 +172,14 @@ class ClockSampler:
 
 
 # DRAM bytes (read + write) per launch, averaged over the 11 weight GEMMs of one
-# 7B step (16384 tokens, N=1, the tuning form: forward bf16x3, backward tf32), all
-# on K3 (the forward's four launches are on K13 now), from one ncu capture of each shape's warm launch:
+# 7B step (16384 tokens, N=1, the tuning form: the forward's four linears on K13 as
+# the bf16 split with their epilogues, seven tf32 products on K3), from one ncu
+# capture of each shape's warm launch:
 #   ncu --metrics dram__bytes_read.sum,dram__bytes_write.sum,gpu__time_duration.sum
-#       --clock-control none -k regex:gemm_kernel --csv
+#       --clock-control none -k "regex:gemm_kernel|linear_" --csv
 #       python -m mround_b200.kernel_sweep --gemm-all 16384
-# (50.8 GB per step for 17.8 GB of operands and outputs).
-GEMM_TRAFFIC_7B = 4.62e9
+# (68.5 GB per step; the same products all on K3, without epilogues, took 50.8).
+GEMM_TRAFFIC_7B = 6.23e9
 
 
 # ----------------------------------------------------------------- workload
@@ -446,7 +447,7 @@ def main():
                      "executed_frac": (exe_flops / (gemm_ms / 1e3) / 1e12) / peak if gemm_ms else 0.0,
                      "gemm_share_of_step": gemm_ms / t_step if t_step else None,
                      "traffic": GEMM_TRAFFIC_7B if args.arch == "qwen2.5-7b" and dist.world == 1 else None,
-                     "traffic_unit": "bytes per weight GEMM as a K3 launch (DRAM read + write), ncu capture of each shape"},
+                     "traffic_unit": "bytes per weight GEMM launch (DRAM read + write), ncu capture of each shape"},
         "clocks": clocks.summary(),
         "e2e": e2e,
     }

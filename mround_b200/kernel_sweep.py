@@ -269,20 +269,40 @@ def gemm_probe(name: str, tokens: int, tf32: bool) -> None:
 
 
 def gemm_all(tokens: int) -> None:
-    """Every weight GEMM of the 7B step in the tuning step's form (forward as
-    the bf16 split, dX and dW as one tf32 product), two launches each in the
-    order of ``gemm_shapes``: under ncu with ``-k regex:gemm_kernel`` the
-    second launch of each pair is the warm one, ``2 * i + 1`` for shape i."""
+    """Every weight GEMM of the 7B step in the tuning step's form (the forward's
+    linears as the bf16 split with their epilogues, dX and dW as one tf32 product),
+    two launches each in the order of ``gemm_shapes``: under ncu with
+    ``-k "regex:gemm_kernel|linear_"`` the second launch of each pair is the warm
+    one, ``2 * i + 1`` for shape i."""
     for name, (m, n, k, ak, bk) in gemm_shapes(tokens).items():
         tf32 = not name.startswith("fwd")
         aop, bop, a_shape, b_shape = _gemm_operands(m, n, k, ak, bk, tf32, "cuda")
         c = torch.empty(m, n, device="cuda")
+        if tf32:
+            def launch():
+                _launch(aop, bop, c, m, n, k, ak, bk, a_shape, b_shape, True)
+        else:
+            launch = _block_linear(name, aop, bop, c)
         for _ in range(2):
-            _launch(aop, bop, c, m, n, k, ak, bk, a_shape, b_shape, tf32)
+            launch()
         torch.cuda.synchronize()
         print(json.dumps({"probe": name, "tokens": tokens, "tf32": tf32, "m": m, "n": n, "k": k}),
               flush=True)
-        del aop, bop, c
+        del aop, bop, c, launch
+
+
+def _block_linear(name: str, x, w, c):
+    """A forward linear as the block calls it: qkv with its bias, o and down with
+    the residual, gate/up with SwiGLU, its pre-activation in ``c``."""
+    m, n = c.shape
+    if name == "fwd_gu":
+        t32 = torch.empty(m, n // 2, device="cuda")
+        return lambda: kernels.linear(x, w, act="swiglu", split=True, pre=c, t32=t32, splits=1)
+    if name == "fwd_qkv":
+        bias = torch.randn(n, device="cuda")
+        return lambda: kernels.linear(x, w, bias=bias, out=c, splits=1)
+    residual = torch.randn(m, n, device="cuda")
+    return lambda: kernels.linear(x, w, residual=residual, out=c, splits=1)
 
 
 def gemm_table(tokens: int, reps: int = 5) -> list[dict]:
