@@ -62,7 +62,7 @@ def reference(x, t, i, temperature):
 @pytest.mark.gpu
 @pytest.mark.parametrize("temperature", [1e-3, 0.1, 1.0, 4.0])
 @pytest.mark.parametrize("v,dtype", [
-    (v, torch.float32) for v in (3e4, 1e8, 1e9, 1e10, 1e12, 1e20, 3e37)] + [
+    (v, torch.float32) for v in (3e4, 1e7, 1.162e7, 1e8, 1e9, 1e10, 1e12, 1e20, 3e37)] + [
     (1e9, torch.bfloat16), (1e10, torch.bfloat16), (1e20, torch.bfloat16), (6e4, torch.float16)])
 def test_rows_far_from_zero(K, v, dtype, temperature):
     """The loss, the gradient, in place and as a pair; whole rows (many) and rows
